@@ -1,0 +1,370 @@
+"""What the training-memory operators are measured on: the AdamW step over many tensors (states in 32 or in 8 bits,
+gradients clipped by their global norm), and the eviction of Gaussians to a budget by accumulated blending weight
+(selection, then the rows of parameters and optimiser states).
+
+A scene is one or several blocks of Gaussians; a block has the six tensors of the model: xyz [P,3], f_dc [P,1,3],
+f_rest [P,M-1,3], opacity [P,1], scaling [P,3], rotation [P,4].  ``run`` computes the plain forms in elementary torch
+operations, or with ``own`` makes the framework's calls."""
+import math
+import random
+import sys
+
+import torch
+
+own = False
+
+BETAS, EPS = (0.9, 0.999), 1e-15
+LRS = (0.00016 * 6.6, 0.0025, 0.0025 / 20, 0.05, 0.005, 0.001)  # the six groups' rates
+M32 = 0xFFFFFFFF
+BLOCK = 64  # elements that share a scale
+
+
+def listed():
+    return [
+        # the smallest scene that is trained on: six launches' worth of latency, no work to speak of
+        {"name": "step32_10k", "op": "step", "bits": 32, "dtype": "float32", "points": 10_000, "blocks": 1, "degree": 0, "clip": False, "decay": 0.0},
+        # an object-sized scene, clipped
+        {"name": "step32_100k_clip", "op": "step", "bits": 32, "dtype": "float32", "points": 100_000, "blocks": 1, "degree": 3, "clip": True, "decay": 0.01},
+        # the headline scene
+        {"name": "step32_1m", "op": "step", "bits": 32, "dtype": "float32", "points": 1_000_000, "blocks": 1, "degree": 3, "clip": False, "decay": 0.0},
+        # a large scene in ragged blocks whose tensors are views of flat buffers, parameters in 16 bits
+        {"name": "step32_blocks_bf16", "op": "step", "bits": 32, "dtype": "bfloat16", "points": 1_500_001, "blocks": 16, "degree": 3, "clip": True, "decay": 0.01},
+        {"name": "step8_10k", "op": "step", "bits": 8, "dtype": "float32", "points": 10_000, "blocks": 1, "degree": 0, "clip": False, "decay": 0.0},
+        {"name": "step8_100k_clip", "op": "step", "bits": 8, "dtype": "float32", "points": 100_000, "blocks": 1, "degree": 3, "clip": True, "decay": 0.01},
+        {"name": "step8_1m", "op": "step", "bits": 8, "dtype": "float32", "points": 1_000_000, "blocks": 1, "degree": 3, "clip": False, "decay": 0.0},
+        # the largest scene: where 8-bit states are wanted
+        {"name": "step8_5m", "op": "step", "bits": 8, "dtype": "float32", "points": 5_000_000, "blocks": 1, "degree": 3, "clip": False, "decay": 0.01},
+        # a small scene loses its tenth
+        {"name": "keep32_10k", "op": "keep", "bits": 32, "points": 10_000, "budget": 9_000, "degree": 0, "protect": False},
+        # the headline scene brought down to half, an odd budget, freshly added rows protected
+        {"name": "keep32_1m", "op": "keep", "bits": 32, "points": 1_000_000, "budget": 500_001, "degree": 3, "protect": True},
+        {"name": "keep8_100k", "op": "keep", "bits": 8, "points": 100_003, "budget": 77_777, "degree": 2, "protect": False},
+        # the largest scene brought down to a budget
+        {"name": "keep8_5m", "op": "keep", "bits": 8, "points": 5_000_000, "budget": 3_000_000, "degree": 3, "protect": True},
+    ]
+
+
+def draw(rng: random.Random):
+    points = int(round(math.exp(rng.uniform(math.log(1000), math.log(2_800_000)))))
+    degree, bits = rng.choice((0, 1, 2, 3, 3)), rng.choice((32, 8))
+    if rng.random() < 0.6:
+        return {"op": "step", "bits": bits, "dtype": rng.choice(("float32", "float32", "bfloat16")), "points": points,
+                "blocks": rng.choice((1, 1, 2, 5, 16)), "degree": degree, "clip": rng.random() < 0.5, "decay": rng.choice((0.0, 0.01))}
+    return {"op": "keep", "bits": bits, "points": points, "budget": int(points * rng.uniform(0.05, 1.0)), "degree": degree,
+            "protect": rng.random() < 0.5}
+
+
+def _shapes(points, degree):
+    return [(points, 3), (points, 1, 3), (points, (degree + 1) ** 2 - 1, 3), (points, 1), (points, 3), (points, 4)]
+
+
+def _block_points(case):
+    """The blocks' sizes: ragged, the same for a case whatever the seed."""
+    n, total = case["blocks"], case["points"]
+    w = [1 + (7 * k * k + 3 * k) % 11 for k in range(n)]
+    got = [total * x // sum(w) for x in w]
+    got[-1] += total - sum(got)
+    return got
+
+
+def _pow2(byte):
+    """2^(byte - 127) of integer tensors."""
+    return torch.where(byte > 0, byte << 23, 0x400000).to(torch.int32).view(torch.float32)
+
+
+def _unpack(codes, scale):
+    n = codes.numel()
+    s = _pow2(scale.view(torch.uint8).to(torch.int32)).repeat_interleave(BLOCK)[:n]
+    return (codes.reshape(-1).to(torch.float32) * s).view(codes.shape)
+
+
+def _pack(x, signed, dither=None):
+    """x [n] in blocks of 64 as e4m3 codes and a power-of-two scale each: the block's largest finite magnitude lands in
+    [128, 256).  ``dither`` (20 bits an element): rounds up where the dropped bits and it carry; None: to nearest even.
+    Without sign nothing but zero rounds to zero."""
+    n = x.numel()
+    bits = x.view(torch.int32)
+    a = bits & 0x7FFFFFFF
+    odd = a >= 0x7F800000
+    full = torch.nn.functional.pad(torch.where(odd, 0, a), (0, -n % BLOCK))
+    byte = ((full.view(-1, BLOCK).amax(1) >> 23) - 7).clamp_min(0)
+    inv = ((254 - byte) << 23).to(torch.int32).view(torch.float32).repeat_interleave(BLOCK)[:n]
+    u = (torch.where(odd, 0, a).view(torch.float32) * inv * 2.0 ** -120).view(torch.int32)
+    up = dither if dither is not None else 0x7FFFF + ((u >> 20) & 1)
+    code = (u + up) >> 20
+    if not signed:
+        code = torch.where((a > 0) & (code == 0), 1, code)
+    code = torch.where(odd, 0x7F, code)
+    if signed:
+        code = code | ((bits >> 24) & 0x80)
+    return code.to(torch.uint8).view(torch.float8_e4m3fn), byte.to(torch.uint8).view(torch.float8_e8m0fnu)
+
+
+def _mix(x):
+    """A 32-bit mixing of x, ints or int64 tensors."""
+    x = x ^ (x >> 16)
+    x = (x * 0x6A09E667) & M32
+    x = x ^ (x >> 15)
+    x = (x * 0xBB67AE85) & M32
+    return x ^ (x >> 16)
+
+
+def _words(n, seed, step, ordinal, device):
+    """32 random bits an element, given by (seed, step, place of the tensor in the list, place of the element)."""
+    key = _mix((_mix((_mix((_mix(seed & M32) + (seed >> 32)) & M32) + step) & M32) + ordinal) & M32)
+    i = torch.arange(n, dtype=torch.int64, device=device)
+    return _mix(((i & M32) * 0x9E3779B9 + (i >> 32) * 0x3C6EF373 + key) & M32)
+
+
+# ------------------------------------------------------------------ inputs
+def prepare(case, seed):
+    dev = torch.device("cuda:0")
+    g = torch.Generator(device=dev).manual_seed(seed)
+
+    def randn(n):
+        return torch.randn(n, generator=g, device=dev)
+
+    if case["op"] == "keep":
+        P = case["points"]
+        shapes = _shapes(P, case["degree"])
+        st = {"case": case, "tensors": [randn(math.prod(s)).view(s) for s in shapes], "states": []}
+        for s in shapes:
+            m = randn(math.prod(s)) * torch.exp(1.5 * randn(math.prod(s))) * 1e-6
+            v = m * m * torch.exp(randn(m.numel()))
+            if case["bits"] == 32:
+                st["states"] += [m.view(s), v.view(s)]
+            else:
+                for x, signed in ((m, True), (v.sqrt(), False)):
+                    codes, scale = _pack(x, signed)
+                    st["states"].append((codes.view(s), scale))
+        # accumulated weights: heavy-tailed, a part never seen (equal zeros: ties), some equal values
+        score = torch.exp(1.5 * randn(P)) * (torch.rand(P, generator=g, device=dev) < 0.8)
+        st["score"] = torch.where(score > 3, torch.round(score), score)
+        st["protect"] = torch.rand(P, generator=g, device=dev) < 0.02 if case["protect"] else None
+        return st
+
+    dtype = getattr(torch, case["dtype"])
+    shapes = [s for P in _block_points(case) for s in _shapes(P, case["degree"])]
+    sizes = [math.prod(s) for s in shapes]
+    n = sum(sizes)
+    flat = case["blocks"] > 1
+    step = int(torch.randint(1, 30_000, (), generator=g, device=dev))
+    st = {"case": case, "step": step, "seed": seed * 1_000_003 + 17, "lr": [LRS[k % 6] for k in range(len(shapes))]}
+
+    def split(x):
+        """Views of one buffer (blocks), or tensors of their own."""
+        parts = [q.view(s) for q, s in zip(x.split(sizes), shapes)]
+        return (x, parts) if flat else (None, [q.clone() for q in parts])
+
+    # gradients over many orders of magnitude; Gaussians outside the view have none
+    seen = (torch.rand((n + 63) // 64, generator=g, device=dev) < 0.6).repeat_interleave(64)[:n]
+    grad = randn(n) * torch.exp(1.5 * randn(n)) * 1e-6
+    m = randn(n) * torch.exp(1.5 * randn(n)) * 3e-7
+    v = (m * m + 1e-14) * torch.exp(1.5 * randn(n))
+    st["p_flat"], st["p"] = split(randn(n).to(dtype))
+    _, st["g"] = split((grad * seen).to(dtype))
+    if case["bits"] == 32:
+        st["m_flat"], ms = split(m)
+        st["v_flat"], vs = split(v)
+        st["states"] = [{"step": step, "exp_avg": a, "exp_avg_sq": b} for a, b in zip(ms, vs)]
+    else:
+        packs = [(_pack(a, True), _pack(b.sqrt(), False)) for a, b in zip(m.split(sizes), v.split(sizes))]
+        cols = {}
+        for k, (who, what) in {"exp_avg": (0, 0), "exp_avg_scale": (0, 1), "exp_rms": (1, 0), "exp_rms_scale": (1, 1)}.items():
+            parts = [q[who][what] for q in packs]
+            if flat:
+                x = torch.cat([q.view(torch.uint8) for q in parts]).view(parts[0].dtype)
+                st[k + "_flat"], parts = x, list(x.split([q.numel() for q in parts]))
+            cols[k] = [q.view(s) if what == 0 else q for q, s in zip(parts, shapes)]
+        st["states"] = [{"step": step, **{k: c[j] for k, c in cols.items()}} for j in range(len(shapes))]
+    return st
+
+
+# ------------------------------------------------------------------ one pass
+def run(st):
+    if own:
+        return _run_own(st)
+    return _keep(st) if st["case"]["op"] == "keep" else _step(st)
+
+
+def _step_outputs(st, norm):
+    keys = ("exp_avg", "exp_avg_sq") if st["case"]["bits"] == 32 else ("exp_avg", "exp_avg_scale", "exp_rms", "exp_rms_scale")
+    if st["p_flat"] is not None:
+        short = {"exp_avg": "m_flat", "exp_avg_sq": "v_flat"} if st["case"]["bits"] == 32 else {k: k + "_flat" for k in keys}
+        out = {"p": st["p_flat"], **{k: st[short[k]] for k in keys}}
+    else:
+        out = {"p": st["p"], **{k: [s[k] for s in st["states"]] for k in keys}}
+    if norm is not None:
+        out["norm"] = norm
+    return out
+
+
+def _max_norm(case):
+    return 1e-6 * math.sqrt(case["points"])  # clips: below the norm of such gradients
+
+
+def _run_own(st):
+    if "3dgs_study_amd" not in sys.path:
+        sys.path.insert(0, "3dgs_study_amd")
+    import train_ops
+
+    case = st["case"]
+    if case["op"] == "keep":
+        rows = train_ops.select_rows(st["score"], case["budget"], st["protect"])
+        taken = train_ops.take_rows(st["tensors"] + st["states"], rows)
+        return {"rows": rows, "taken": taken}
+    norm = scale = None
+    if case["clip"]:
+        norm, scale = train_ops.grad_norm(st["g"], _max_norm(case))
+    train_ops.adamw_step(st["p"], st["g"], st["states"], st["lr"], weight_decay=case["decay"], betas=BETAS, eps=EPS,
+                         grad_scale=scale, seed=st["seed"])
+    return _step_outputs(st, norm)
+
+
+def _step(st):
+    case, (b1, b2) = st["case"], BETAS
+    norm = scale = None
+    if case["clip"]:
+        total = sum(g.to(torch.float64).square().sum() for g in st["g"])
+        norm64 = total.sqrt()
+        norm = norm64.to(torch.float32)
+        scale = (_max_norm(case) / (norm64 + 1e-6)).clamp_max(1.0).to(torch.float32)
+    for k, (p, g, s, lr) in enumerate(zip(st["p"], st["g"], st["states"], st["lr"])):
+        s["step"] += 1
+        t = s["step"]
+        n = p.numel()
+        decay, neg_step = 1.0 - lr * case["decay"], -lr / (1.0 - b1 ** t)
+        inv_bc2 = 1.0 / math.sqrt(1.0 - b2 ** t)
+        w = None
+        if case["bits"] == 8 or p.dtype == torch.bfloat16:
+            w = _words(n, st["seed"], t, k, p.device)
+        x = g.reshape(-1).to(torch.float32)
+        if scale is not None:
+            x = x * scale
+        if case["bits"] == 32:
+            m, v = s["exp_avg"].view(-1), s["exp_avg_sq"].view(-1)
+        else:
+            m = _unpack(s["exp_avg"], s["exp_avg_scale"]).view(-1)
+            r = _unpack(s["exp_rms"], s["exp_rms_scale"]).view(-1)
+            v = r * r
+        m2 = m + (x - m) * (1.0 - b1)
+        v2 = v * b2 + (x * x) * (1.0 - b2)
+        r2 = v2.sqrt()
+        p2 = p.view(-1).to(torch.float32) * decay + (m2 / (r2 * inv_bc2 + EPS)) * neg_step
+        if p.dtype == torch.bfloat16:
+            low = ((w * 0x9E3779B9) & M32) >> 16
+            bits = p2.view(torch.int32)
+            p2 = torch.where(torch.isfinite(p2), (bits + low.to(torch.int32)) & -0x10000, bits).view(torch.float32)
+        p.view(-1).copy_(p2)
+        if case["bits"] == 32:
+            m.copy_(m2)
+            v.copy_(v2)
+        else:
+            d1, d2 = ((w >> 16) << 4 | 8).to(torch.int32), ((w & 0xFFFF) << 4 | 8).to(torch.int32)
+            for key, y, signed, d in (("exp_avg", m2, True, d1), ("exp_rms", r2, False, d2)):
+                codes, e = _pack(y, signed, d)
+                s[key].view(torch.uint8).view(-1).copy_(codes.view(torch.uint8))
+                s[key + "_scale"].view(torch.uint8).copy_(e.view(torch.uint8))
+    return _step_outputs(st, norm)
+
+
+def _select(score, budget, protect):
+    b = (score + 0.0).view(torch.int32).to(torch.int64)
+    key = torch.where(b >= 0, b, -(b & 0x7FFFFFFF))
+    key = torch.where(torch.isnan(score), -(1 << 40), key)
+    if protect is not None:
+        key = torch.where(protect, 1 << 40, key)
+    order = torch.sort(key, descending=True, stable=True).indices[:budget]
+    return torch.sort(order).values
+
+
+def _keep(st):
+    rows = _select(st["score"], st["case"]["budget"], st["protect"])
+    taken = [t.index_select(0, rows) for t in st["tensors"]]
+    for k, s in enumerate(st["states"]):
+        if isinstance(s, tuple):
+            x = _unpack(*s).index_select(0, rows)
+            codes, scale = _pack(x.reshape(-1), signed=k % 2 == 0)
+            taken.append((codes.view(x.shape), scale))
+        else:
+            taken.append(s.index_select(0, rows))
+    return {"rows": rows, "taken": taken}
+
+
+# ------------------------------------------------------------------ 64 bits
+def _blocks64(x):
+    """(x in units of its block's scale, the scales), from the definition: the scale is the power of two that brings the
+    block's largest magnitude to [128, 256), and 2^-127 at least."""
+    full = torch.nn.functional.pad(x, (0, -x.numel() % BLOCK)).view(-1, BLOCK)
+    s = torch.frexp(full.abs().amax(1))[1].to(torch.float64) - 8
+    s = torch.exp2(torch.where(full.abs().amax(1) > 0, s, -127.0).clamp_min(-127.0))
+    return (full / s[:, None]).view(-1)[: x.numel()], s
+
+
+def _value64(codes, scale):
+    return codes.to(torch.float64).view(-1) * scale.to(torch.float64).repeat_interleave(BLOCK)[: codes.numel()]
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    if case["op"] == "keep":
+        score = st["score"].to(torch.float64)
+        if st["protect"] is not None:
+            score = score.masked_fill(st["protect"], math.inf)
+        first = torch.sort(score, descending=True, stable=True).indices[: case["budget"]]
+        kept = torch.zeros(case["points"], dtype=torch.bool, device=score.device)
+        kept[first] = True
+        out = [t[kept].to(torch.float64) for t in st["tensors"]]
+        for s in st["states"]:
+            if isinstance(s, tuple):
+                x = _value64(*s).view(s[0].shape)[kept]
+                codes, e = _blocks64(x.reshape(-1))
+                out.append((codes.view(x.shape), e))
+            else:
+                out.append(s[kept].to(torch.float64))
+        return {"rows": kept.nonzero().view(-1), "taken": out}
+    b1, b2 = BETAS
+    t = st["step"] + 1
+    out = {"p": [], "exp_avg": [], **({"exp_avg_sq": []} if case["bits"] == 32 else {"exp_avg_scale": [], "exp_rms": [], "exp_rms_scale": []})}
+    norm, c = None, 1.0
+    if case["clip"]:
+        norm = torch.cat([g.reshape(-1) for g in st["g"]]).to(torch.float64).norm()
+        c = torch.clamp(_max_norm(case) / (norm + 1e-6), max=1.0)
+    for p, g, s, lr in zip(st["p"], st["g"], st["states"], st["lr"]):
+        x = c * g.to(torch.float64).reshape(-1)
+        if case["bits"] == 32:
+            m, v = s["exp_avg"].to(torch.float64).view(-1), s["exp_avg_sq"].to(torch.float64).view(-1)
+        else:
+            m = _value64(s["exp_avg"], s["exp_avg_scale"])
+            v = _value64(s["exp_rms"], s["exp_rms_scale"]) ** 2
+        m = b1 * m + (1 - b1) * x
+        v = b2 * v + (1 - b2) * x ** 2
+        q = p.to(torch.float64).view(-1)
+        q = q - lr * case["decay"] * q - lr * (m / (1 - b1 ** t)) / (torch.sqrt(v / (1 - b2 ** t)) + EPS)
+        out["p"].append(q.view(p.shape))
+        if case["bits"] == 32:
+            out["exp_avg"].append(m.view(p.shape))
+            out["exp_avg_sq"].append(v.view(p.shape))
+        else:
+            for key, y in (("exp_avg", m), ("exp_rms", v.sqrt())):
+                codes, e = _blocks64(y)
+                out[key].append(codes.view(p.shape))
+                out[key + "_scale"].append(e)
+    if case["blocks"] > 1:
+        out = {k: torch.cat([x.reshape(-1) for x in v]) for k, v in out.items()}
+    if norm is not None:
+        out["norm"] = norm
+    return out
+
+
+# ------------------------------------------------------------------ work
+def work(case):
+    per = sum(math.prod(s[1:]) for s in _shapes(1, case["degree"]))
+    if case["op"] == "keep":
+        row = per * (12 if case["bits"] == 32 else 6 + 2 / BLOCK)
+        P, K = case["points"], case["budget"]
+        return {"bytes": P * (5 if case["protect"] else 4) + 8 * K + 2 * K * row, "flops": float(P)}
+    n = case["points"] * per
+    p = 2 if case["dtype"] == "bfloat16" else 4
+    state = 16 if case["bits"] == 32 else 4 * (1 + 1 / BLOCK)
+    return {"bytes": n * (3 * p + state), "flops": n * (15.0 + (2.0 if case["clip"] else 0.0))}
