@@ -131,12 +131,11 @@ def prepare(case, seed):
         for s in shapes:
             m = randn(math.prod(s)) * torch.exp(1.5 * randn(math.prod(s))) * 1e-6
             v = m * m * torch.exp(randn(m.numel()))
-            if case["bits"] == 32:
-                st["states"] += [m.view(s), v.view(s)]
-            else:
-                for x, signed in ((m, True), (v.sqrt(), False)):
-                    codes, scale = _pack(x, signed)
-                    st["states"].append((codes.view(s), scale))
+            state = {"step": 7, "exp_avg": m.view(s), "exp_avg_sq": v.view(s)}
+            if case["bits"] == 8:
+                (a, ea), (r, er) = _pack(m, True), _pack(v.sqrt(), False)
+                state = {"step": 7, "exp_avg": a.view(s), "exp_avg_scale": ea, "exp_rms": r.view(s), "exp_rms_scale": er}
+            st["states"].append(state)
         # accumulated weights: heavy-tailed, a part never seen (equal zeros: ties), some equal values
         score = torch.exp(1.5 * randn(P)) * (torch.rand(P, generator=g, device=dev) < 0.8)
         st["score"] = torch.where(score > 3, torch.round(score), score)
@@ -211,8 +210,8 @@ def _run_own(st):
     case = st["case"]
     if case["op"] == "keep":
         rows = train_ops.select_rows(st["score"], case["budget"], st["protect"])
-        taken = train_ops.take_rows(st["tensors"] + st["states"], rows)
-        return {"rows": rows, "taken": taken}
+        tensors, states = train_ops.take_rows(st["tensors"], rows, states=st["states"])
+        return {"rows": rows, "tensors": tensors, "states": [{k: x for k, x in s.items() if k != "step"} for s in states]}
     norm = scale = None
     if case["clip"]:
         norm, scale = train_ops.grad_norm(st["g"], _max_norm(case))
@@ -280,15 +279,18 @@ def _select(score, budget, protect):
 
 def _keep(st):
     rows = _select(st["score"], st["case"]["budget"], st["protect"])
-    taken = [t.index_select(0, rows) for t in st["tensors"]]
-    for k, s in enumerate(st["states"]):
-        if isinstance(s, tuple):
-            x = _unpack(*s).index_select(0, rows)
-            codes, scale = _pack(x.reshape(-1), signed=k % 2 == 0)
-            taken.append((codes.view(x.shape), scale))
-        else:
-            taken.append(s.index_select(0, rows))
-    return {"rows": rows, "taken": taken}
+    states = []
+    for s in st["states"]:
+        if "exp_avg_sq" in s:
+            states.append({k: s[k].index_select(0, rows) for k in ("exp_avg", "exp_avg_sq")})
+            continue
+        got = {}
+        for key, signed in (("exp_avg", True), ("exp_rms", False)):
+            x = _unpack(s[key], s[key + "_scale"]).index_select(0, rows)
+            codes, got[key + "_scale"] = _pack(x.reshape(-1), signed)
+            got[key] = codes.view(x.shape)
+        states.append(got)
+    return {"rows": rows, "tensors": [t.index_select(0, rows) for t in st["tensors"]], "states": states}
 
 
 # ------------------------------------------------------------------ 64 bits
@@ -314,15 +316,18 @@ def exact(case, seed):
         first = torch.sort(score, descending=True, stable=True).indices[: case["budget"]]
         kept = torch.zeros(case["points"], dtype=torch.bool, device=score.device)
         kept[first] = True
-        out = [t[kept].to(torch.float64) for t in st["tensors"]]
+        states = []
         for s in st["states"]:
-            if isinstance(s, tuple):
-                x = _value64(*s).view(s[0].shape)[kept]
-                codes, e = _blocks64(x.reshape(-1))
-                out.append((codes.view(x.shape), e))
-            else:
-                out.append(s[kept].to(torch.float64))
-        return {"rows": kept.nonzero().view(-1), "taken": out}
+            if "exp_avg_sq" in s:
+                states.append({k: s[k][kept].to(torch.float64) for k in ("exp_avg", "exp_avg_sq")})
+                continue
+            got = {}
+            for key in ("exp_avg", "exp_rms"):
+                x = _value64(s[key], s[key + "_scale"]).view(s[key].shape)[kept]
+                codes, got[key + "_scale"] = _blocks64(x.reshape(-1))
+                got[key] = codes.view(x.shape)
+            states.append(got)
+        return {"rows": kept.nonzero().view(-1), "tensors": [t[kept].to(torch.float64) for t in st["tensors"]], "states": states}
     b1, b2 = BETAS
     t = st["step"] + 1
     out = {"p": [], "exp_avg": [], **({"exp_avg_sq": []} if case["bits"] == 32 else {"exp_avg_scale": [], "exp_rms": [], "exp_rms_scale": []})}
