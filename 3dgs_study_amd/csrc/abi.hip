@@ -896,6 +896,71 @@ int gsr_densify_stats(int32_t P, const int32_t *radii, const float *viewspace_gr
                      "densify_stats");
 }
 
+int gsr_adamw_step(const gsr_adamw_segment *segs, int32_t nseg, int32_t dtype, int32_t state_bits, double beta1,
+                   double beta2, double eps, const float *grad_scale, uint64_t seed, void *stream) {
+    if (nseg < 0 || (nseg > 0 && !segs)) return fail(GSR_ERR_ARGS, "adamw: bad segment list (%d)", nseg);
+    if (dtype != GSR_DTYPE_F32 && dtype != GSR_DTYPE_BF16) return fail(GSR_ERR_ARGS, "adamw: unknown dtype %d", dtype);
+    if (state_bits != 32 && state_bits != 8) return fail(GSR_ERR_ARGS, "adamw: state_bits must be 32 or 8 (got %d)", state_bits);
+    if (!(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0))
+        return fail(GSR_ERR_ARGS, "adamw: betas must be in [0, 1) and eps >= 0");
+    for (int k = 0; k < nseg; k++) {
+        const gsr_adamw_segment &q = segs[k];
+        if (q.n < 0 || q.n > (int64_t)1 << 33) return fail(GSR_ERR_ARGS, "adamw: bad size %lld in segment %d", (long long)q.n, k);
+        if (q.step < 1) return fail(GSR_ERR_ARGS, "adamw: step must be >= 1 (got %d)", q.step);
+        if (q.n > 0 && (!q.param || !q.grad || !q.exp_avg || !q.exp_second || (state_bits == 8 && (!q.avg_scale || !q.second_scale))))
+            return fail(GSR_ERR_ARGS, "adamw: NULL buffer in segment %d", k);
+    }
+    return check_hip(launch_adamw(segs, nseg, dtype, state_bits, beta1, beta2, eps, grad_scale, seed, (hipStream_t)stream),
+                     "adamw");
+}
+
+size_t gsr_grad_norm_scratch_bytes(int32_t nseg) { return nseg > 0 ? grad_norm_scratch_bytes(nseg) : 8; }
+
+int gsr_grad_norm(const gsr_grad_segment *segs, int32_t nseg, double max_norm, void *scratch, float *out,
+                  void *stream) {
+    if (nseg < 0 || (nseg > 0 && !segs)) return fail(GSR_ERR_ARGS, "grad_norm: bad segment list (%d)", nseg);
+    if (!(max_norm >= 0)) return fail(GSR_ERR_ARGS, "grad_norm: max_norm must be >= 0");
+    if (!scratch || !out) return fail(GSR_ERR_ARGS, "grad_norm: NULL buffer");
+    for (int k = 0; k < nseg; k++) {
+        if (segs[k].n < 0 || segs[k].n > (int64_t)1 << 33)
+            return fail(GSR_ERR_ARGS, "grad_norm: bad size %lld in segment %d", (long long)segs[k].n, k);
+        if (segs[k].dtype != GSR_DTYPE_F32 && segs[k].dtype != GSR_DTYPE_BF16)
+            return fail(GSR_ERR_ARGS, "grad_norm: unknown dtype %d", segs[k].dtype);
+        if (segs[k].n > 0 && !segs[k].grad) return fail(GSR_ERR_ARGS, "grad_norm: NULL buffer in segment %d", k);
+    }
+    return check_hip(launch_grad_norm(segs, nseg, max_norm, scratch, out, (hipStream_t)stream), "grad_norm");
+}
+
+size_t gsr_select_rows_scratch_bytes(int32_t P) { return P > 0 ? select_rows_scratch_bytes(P) : 0; }
+
+int gsr_select_rows(const float *score, const uint8_t *protect, int32_t P, int32_t budget, int64_t *rows,
+                    void *scratch, void *stream) {
+    if (P < 0 || budget < 0) return fail(GSR_ERR_ARGS, "select_rows: bad P %d / budget %d", P, budget);
+    if (P == 0 || budget == 0) return GSR_OK;
+    if (!score || !rows || !scratch) return fail(GSR_ERR_ARGS, "select_rows: NULL buffer");
+    return check_hip(launch_select_rows(score, protect, P, budget < P ? budget : P, rows, scratch, (hipStream_t)stream),
+                     "select_rows");
+}
+
+int gsr_take_rows(const gsr_rows_segment *segs, int32_t nseg, int64_t P, const int64_t *rows, int64_t K,
+                  void *stream) {
+    if (nseg < 0 || (nseg > 0 && !segs)) return fail(GSR_ERR_ARGS, "take_rows: bad segment list (%d)", nseg);
+    if (P < 0 || K < 0 || K > INT32_MAX) return fail(GSR_ERR_ARGS, "take_rows: bad P %lld / K %lld", (long long)P, (long long)K);
+    if (K == 0) return GSR_OK;
+    if (!rows) return fail(GSR_ERR_ARGS, "take_rows: NULL rows");
+    for (int k = 0; k < nseg; k++) {
+        const gsr_rows_segment &q = segs[k];
+        if (q.kind < GSR_ROWS_PLAIN || q.kind > GSR_ROWS_E4M3_SIGNED)
+            return fail(GSR_ERR_ARGS, "take_rows: unknown kind %d in segment %d", q.kind, k);
+        const int64_t most = (int64_t)1 << (q.kind == GSR_ROWS_PLAIN ? 34 : 33);
+        if (q.row_bytes < 0 || q.row_bytes >= (int64_t)1 << 30 || (q.row_bytes && K > most / q.row_bytes))
+            return fail(GSR_ERR_ARGS, "take_rows: rows of %lld bytes in segment %d", (long long)q.row_bytes, k);
+        if (q.row_bytes && (!q.dst || (P > 0 && !q.src) || (q.kind != GSR_ROWS_PLAIN && (!q.dst_scale || (P > 0 && !q.src_scale)))))
+            return fail(GSR_ERR_ARGS, "take_rows: NULL buffer in segment %d", k);
+    }
+    return check_hip(launch_take_rows(segs, nseg, P, rows, K, (hipStream_t)stream), "take_rows");
+}
+
 size_t gsr_knn_scratch_bytes(int32_t P) { return P > 0 ? knn_scratch_bytes(P) : 0; }
 
 int gsr_knn_mean_dist2(int32_t P, const float *points, float *dist2, void *scratch, void *stream) {

@@ -1,0 +1,336 @@
+// adamw.hip — the AdamW step over any number of tensors, with its two moments in 32
+// bits or in 8, and the global gradient norm that clips it.
+//
+//   g' = c g                                    c: the clip coefficient, on the device
+//   m' = m + (1 - b1) (g' - m)                  v' = b2 v + (1 - b2) g'^2
+//   p' = p (1 - lr wd) - lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+//
+// The operations are those of torch.optim.AdamW in its order, in fp32, except that
+// the bias correction of the root is a product with its reciprocal.
+//
+// 8-bit states hold m and r = sqrt(v) (half the range of v's exponents) as e4m3 codes
+// with a power-of-two scale for every 64 elements (gsr_blockscale.hpp).  They are
+// rounded stochastically: an e4m3 step is 6-12 % of the value, one update moves v by
+// (1 - b2) = 0.1 %, so rounding to nearest would never let a second moment fall, and
+// would hold the first moments of Gaussians that no view sees at their last few codes,
+// which then drift for ever.  The parameter is updated from the fp32 moments before
+// they are rounded.
+//
+// Parameters and gradients are fp32 or bf16; a bf16 parameter is rounded
+// stochastically too (an update below 2^-9 of the parameter would be lost).
+#include <cmath>
+
+#include "gsr_blockscale.hpp"
+#include "gsr_kernels.hpp"
+
+// every product and sum rounds by itself, as in the formulas above: the codes then do
+// not depend on which of them the compiler would have fused
+#pragma clang fp contract(off)
+
+namespace gsr {
+
+constexpr int AW_THREADS = 256, AW_VEC = 4, AW_SEGS = 40;  // 40 segments: 3.1 KB of kernel arguments
+constexpr int AW_TILE = AW_THREADS * AW_VEC;               // elements per workgroup
+
+struct AdamWSeg {
+    void *p;
+    const void *g;
+    void *m, *v;           // float, or e4m3 codes of m and sqrt(v)
+    uint8_t *ms, *vs;      // their scales
+    int64_t n;
+    float decay, neg_step, inv_bc2;
+    uint32_t key;
+};
+struct AdamWArgs {
+    int nseg;
+    float w1, b2, w2, eps;
+    const float *scale;  // NULL: 1
+    int block0[AW_SEGS + 1];
+    AdamWSeg seg[AW_SEGS];
+};
+
+template <typename T>
+struct Elems;
+template <>
+struct Elems<float> {
+    static __device__ __forceinline__ void load4(const float *s, float x[4]) {
+        const f32x4_u v = *reinterpret_cast<const f32x4_u *>(s);
+        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    }
+    static __device__ __forceinline__ float load(const float *s) { return *s; }
+    static __device__ __forceinline__ float round(float x, uint32_t) { return x; }
+    static __device__ __forceinline__ void store4(float *d, const float x[4]) {
+        f32x4_u v = {x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4_u *>(d) = v;
+    }
+    static __device__ __forceinline__ void store(float *d, float x) { *d = x; }
+};
+template <>
+struct Elems<uint16_t> {  // bf16
+    static __device__ __forceinline__ void load4(const uint16_t *s, float x[4]) {
+        const u16x4_u v = *reinterpret_cast<const u16x4_u *>(s);
+        x[0] = as_f32((uint32_t)v.x << 16), x[1] = as_f32((uint32_t)v.y << 16);
+        x[2] = as_f32((uint32_t)v.z << 16), x[3] = as_f32((uint32_t)v.w << 16);
+    }
+    static __device__ __forceinline__ float load(const uint16_t *s) { return as_f32((uint32_t)*s << 16); }
+    // 16 more bits of the element's word (the moments take its halves) decide the rounding
+    static __device__ __forceinline__ float round(float x, uint32_t word) {
+        const uint32_t b = as_u32(x);
+        if ((b & 0x7F800000u) == 0x7F800000u) return as_f32(b | ((b & 0x7FFFFFu) ? 0x400000u : 0u));  // a NaN stays one
+        return as_f32(b + ((word * 0x9E3779B9u) >> 16));
+    }
+    static __device__ __forceinline__ void store4(uint16_t *d, const float x[4]) {
+        u16x4_u v = {(uint16_t)(as_u32(x[0]) >> 16), (uint16_t)(as_u32(x[1]) >> 16), (uint16_t)(as_u32(x[2]) >> 16),
+                     (uint16_t)(as_u32(x[3]) >> 16)};
+        *reinterpret_cast<u16x4_u *>(d) = v;
+    }
+    static __device__ __forceinline__ void store(uint16_t *d, float x) { *d = (uint16_t)(as_u32(x) >> 16); }
+};
+
+// the segment of a workgroup: the last one that starts at or before it
+__device__ __forceinline__ int segment_of(const int *block0, int nseg, int b) {
+    int lo = 0, hi = nseg;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (block0[mid] <= b) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ void adamw_one(const AdamWArgs &a, const AdamWSeg &s, float c, float &p, float g, float &m,
+                                          float &v, float &r) {
+    const float x = g * c;
+    m = m + (x - m) * a.w1;
+    v = v * a.b2 + (x * x) * a.w2;
+    r = sqrtf(v);
+    p = p * s.decay + (m / (r * s.inv_bc2 + a.eps)) * s.neg_step;
+}
+
+template <typename T, bool BITS8>
+__global__ void __launch_bounds__(AW_THREADS) adamw_kernel(AdamWArgs a) {
+    const int k = segment_of(a.block0, a.nseg, (int)blockIdx.x);
+    const AdamWSeg &s = a.seg[k];
+    const int64_t n = s.n, i = (int64_t)((int)blockIdx.x - a.block0[k]) * AW_TILE + threadIdx.x * AW_VEC;
+    const float c = a.scale ? *a.scale : 1.f;
+    const int live = (int)(n - i < AW_VEC ? (n - i > 0 ? n - i : 0) : AW_VEC);
+    T *p = (T *)s.p + i;
+    const T *g = (const T *)s.g + i;
+    float P[4] = {0, 0, 0, 0}, G[4] = {0, 0, 0, 0}, M[4] = {0, 0, 0, 0}, V[4] = {0, 0, 0, 0}, R[4];
+    if (live == AW_VEC) {
+        Elems<T>::load4(p, P);
+        Elems<T>::load4(g, G);
+    } else {
+        for (int j = 0; j < live; j++) P[j] = Elems<T>::load(p + j), G[j] = Elems<T>::load(g + j);
+    }
+    if (BITS8) {
+        uint8_t *mc = (uint8_t *)s.m + i, *rc = (uint8_t *)s.v + i;
+        uint32_t mw = 0, rw = 0, mb = 0, rb = 0;
+        if (live) mb = s.ms[i / SCALE_BLOCK], rb = s.vs[i / SCALE_BLOCK];
+        if (live == AW_VEC) {
+            mw = *reinterpret_cast<const u32_u *>(mc), rw = *reinterpret_cast<const u32_u *>(rc);
+        } else {
+            for (int j = 0; j < live; j++) mw |= (uint32_t)mc[j] << 8 * j, rw |= (uint32_t)rc[j] << 8 * j;
+        }
+        e4m3_decode4(mw, M);
+        e4m3_decode4(rw, R);
+        const float msc = block_scale(mb), rsc = block_scale(rb);
+        uint32_t ma = 0, ra = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            M[j] *= msc;
+            R[j] *= rsc;
+            V[j] = R[j] * R[j];
+            adamw_one(a, s, c, P[j], G[j], M[j], V[j], R[j]);
+            ma = max(ma, j < live ? coded_bits(M[j]) : 0u);
+            ra = max(ra, j < live ? coded_bits(R[j]) : 0u);
+        }
+        mb = scale_byte(row_max(ma));
+        rb = scale_byte(row_max(ra));
+        mw = rw = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t w = dither_word((uint64_t)(i + j), s.key);
+            mw |= e4m3_stochastic<true>(M[j], mb, w >> 16) << 8 * j;
+            rw |= e4m3_stochastic<false>(R[j], rb, w & 0xFFFFu) << 8 * j;
+            P[j] = Elems<T>::round(P[j], w);
+        }
+        if (live == AW_VEC) {
+            *reinterpret_cast<u32_u *>(mc) = mw;
+            *reinterpret_cast<u32_u *>(rc) = rw;
+        } else {
+            for (int j = 0; j < live; j++) mc[j] = (uint8_t)(mw >> 8 * j), rc[j] = (uint8_t)(rw >> 8 * j);
+        }
+        if (live && (threadIdx.x & 15) == 0) s.ms[i / SCALE_BLOCK] = (uint8_t)mb, s.vs[i / SCALE_BLOCK] = (uint8_t)rb;
+    } else {
+        float *m = (float *)s.m + i, *v = (float *)s.v + i;
+        if (live == AW_VEC) {
+            Elems<float>::load4(m, M);
+            Elems<float>::load4(v, V);
+        } else {
+            for (int j = 0; j < live; j++) M[j] = m[j], V[j] = v[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            adamw_one(a, s, c, P[j], G[j], M[j], V[j], R[j]);
+            if (sizeof(T) == 2) P[j] = Elems<T>::round(P[j], dither_word((uint64_t)(i + j), s.key));
+        }
+        if (live == AW_VEC) {
+            Elems<float>::store4(m, M);
+            Elems<float>::store4(v, V);
+        } else {
+            for (int j = 0; j < live; j++) m[j] = M[j], v[j] = V[j];
+        }
+    }
+    if (live == AW_VEC) {
+        Elems<T>::store4(p, P);
+    } else {
+        for (int j = 0; j < live; j++) Elems<T>::store(p + j, P[j]);
+    }
+}
+
+hipError_t launch_adamw(const gsr_adamw_segment *segs, int nseg, int dtype, int state_bits, double beta1, double beta2,
+                        double eps, const float *grad_scale, uint64_t seed, hipStream_t st) {
+    AdamWArgs a;
+    a.w1 = (float)(1.0 - beta1);
+    a.b2 = (float)beta2;
+    a.w2 = (float)(1.0 - beta2);
+    a.eps = (float)eps;
+    a.scale = grad_scale;
+    for (int k = 0; k < nseg;) {
+        int blocks = 0;
+        a.nseg = 0;
+        for (; k < nseg && a.nseg < AW_SEGS; k++) {
+            const gsr_adamw_segment &q = segs[k];
+            const int64_t b = (q.n + AW_TILE - 1) / AW_TILE;
+            if (b == 0) continue;
+            if (blocks && blocks + b > GSR_MAX_BLOCKS) break;  // the next launch takes it
+            AdamWSeg &s = a.seg[a.nseg];
+            s.p = q.param, s.g = q.grad, s.m = q.exp_avg, s.v = q.exp_second;
+            s.ms = q.avg_scale, s.vs = q.second_scale;
+            s.n = q.n;
+            s.decay = (float)(1.0 - q.lr * q.weight_decay);
+            s.neg_step = (float)(-q.lr / (1.0 - std::pow(beta1, q.step)));
+            s.inv_bc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, q.step)));
+            s.key = dither_key(seed, (uint32_t)q.step, (uint32_t)q.ordinal);
+            a.block0[a.nseg++] = blocks;
+            blocks += (int)b;
+        }
+        if (!a.nseg) continue;
+        a.block0[a.nseg] = blocks;
+        const dim3 g(blocks), t(AW_THREADS);
+        if (dtype == GSR_DTYPE_F32 && state_bits == 32) hipLaunchKernelGGL((adamw_kernel<float, false>), g, t, 0, st, a);
+        else if (dtype == GSR_DTYPE_F32) hipLaunchKernelGGL((adamw_kernel<float, true>), g, t, 0, st, a);
+        else if (state_bits == 32) hipLaunchKernelGGL((adamw_kernel<uint16_t, false>), g, t, 0, st, a);
+        else hipLaunchKernelGGL((adamw_kernel<uint16_t, true>), g, t, 0, st, a);
+        if (hipError_t e = hipGetLastError()) return e;
+    }
+    return hipSuccess;
+}
+
+// ------------------------------------------------------------ global gradient norm
+//
+// norm = sqrt(sum g^2) over all tensors, c = min(1, max_norm / (norm + 1e-6)).  Squares
+// and sums in 64 bits (the fp64 rate is far above what the stream of gradients needs):
+// no overflow, and the same value whatever the split.  Each workgroup leaves one partial
+// sum; one workgroup adds them in a fixed order.
+constexpr int GN_THREADS = 256, GN_SEGS = 128, GN_BLOCKS = 2048;
+constexpr int GN_TILE = GN_THREADS * 4 * 4;
+struct NormArgs {
+    int nseg, tiles;
+    double *partials;
+    int tile0[GN_SEGS + 1];
+    gsr_grad_segment seg[GN_SEGS];
+};
+
+template <typename T>
+__device__ __forceinline__ double square_sum(const T *g, int64_t n) {
+    double acc = 0;
+    if (n >= GN_TILE) {
+        float x[4][4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) Elems<T>::load4(g + (u * GN_THREADS + threadIdx.x) * 4, x[u]);
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc = __builtin_fma((double)x[u][j], (double)x[u][j], acc);
+    } else {
+        for (int64_t i = threadIdx.x; i < n; i += GN_THREADS) {
+            const double x = (double)Elems<T>::load(g + i);
+            acc = __builtin_fma(x, x, acc);
+        }
+    }
+    return acc;
+}
+
+template <int THREADS>
+__device__ __forceinline__ double block_sum_f64(double v, double *red) {
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double t = 0;
+    for (int k = 0; k < THREADS / 64; k++) t += red[k];
+    return t;
+}
+
+__global__ void __launch_bounds__(GN_THREADS) grad_norm_kernel(NormArgs a) {
+    __shared__ double red[GN_THREADS / 64];
+    double acc = 0;
+    for (int t = blockIdx.x; t < a.tiles; t += gridDim.x) {
+        const int k = segment_of(a.tile0, a.nseg, t);
+        const gsr_grad_segment &s = a.seg[k];
+        const int64_t i = (int64_t)(t - a.tile0[k]) * GN_TILE;
+        acc += s.dtype == GSR_DTYPE_F32 ? square_sum((const float *)s.grad + i, s.n - i)
+                                        : square_sum((const uint16_t *)s.grad + i, s.n - i);
+    }
+    const double t = block_sum_f64<GN_THREADS>(acc, red);
+    if (threadIdx.x == 0) a.partials[blockIdx.x] = t;
+}
+
+constexpr int GNF_THREADS = 1024;
+__global__ void __launch_bounds__(GNF_THREADS) grad_norm_finish_kernel(const double *partials, int n, double max_norm,
+                                                                       float *out) {
+    __shared__ double red[GNF_THREADS / 64];
+    double acc = 0;
+    for (int i = threadIdx.x; i < n; i += GNF_THREADS) acc += partials[i];
+    const double norm = sqrt(block_sum_f64<GNF_THREADS>(acc, red));
+    if (threadIdx.x == 0) {
+        const double c = max_norm / (norm + 1e-6);
+        out[0] = (float)norm;
+        out[1] = c >= 1.0 ? 1.f : (float)c;  // a NaN norm stays NaN, as an infinite one gives 0
+    }
+}
+
+size_t grad_norm_scratch_bytes(int nseg) {
+    return (size_t)((nseg + GN_SEGS - 1) / GN_SEGS) * GN_BLOCKS * sizeof(double);
+}
+
+hipError_t launch_grad_norm(const gsr_grad_segment *segs, int nseg, double max_norm, void *scratch, float *out,
+                            hipStream_t st) {
+    NormArgs a;
+    int parts = 0;
+    for (int k = 0; k < nseg;) {
+        a.nseg = 0, a.tiles = 0;
+        // a launch takes GN_SEGS entries of the list, empty ones too: the scratch holds one
+        // set of partial sums for each
+        for (int q = 0; q < GN_SEGS && k < nseg; q++, k++) {
+            const int64_t t = (segs[k].n + GN_TILE - 1) / GN_TILE;
+            if (t == 0) continue;
+            a.seg[a.nseg] = segs[k];
+            a.tile0[a.nseg++] = a.tiles;
+            a.tiles += (int)t;
+        }
+        if (!a.nseg) continue;
+        a.tile0[a.nseg] = a.tiles;
+        const int blocks = a.tiles < GN_BLOCKS ? a.tiles : GN_BLOCKS;
+        a.partials = (double *)scratch + parts;
+        parts += blocks;
+        hipLaunchKernelGGL(grad_norm_kernel, dim3(blocks), dim3(GN_THREADS), 0, st, a);
+        if (hipError_t e = hipGetLastError()) return e;
+    }
+    hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(GNF_THREADS), 0, st, (const double *)scratch, parts,
+                       max_norm, out);
+    return hipGetLastError();
+}
+
+}  // namespace gsr

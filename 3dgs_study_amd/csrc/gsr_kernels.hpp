@@ -110,6 +110,24 @@ hipError_t launch_adam(const gsr_adam_segment *segs, int nseg, int step, double 
 hipError_t launch_densify_stats(int P, const int32_t *radii, const float *vgrad, int vstride, float *max_radii,
                                 float *grad_accum, float *denom, hipStream_t s);
 
+// Workgroups that one launch of 256-thread workgroups may have (a grid holds fewer than
+// 2^32 work items); the launchers over many segments start another launch beyond it
+constexpr int64_t GSR_MAX_BLOCKS = (1 << 24) - 1;
+
+// adamw.hip
+hipError_t launch_adamw(const gsr_adamw_segment *segs, int nseg, int dtype, int state_bits, double beta1, double beta2,
+                        double eps, const float *grad_scale, uint64_t seed, hipStream_t s);
+size_t grad_norm_scratch_bytes(int nseg);
+hipError_t launch_grad_norm(const gsr_grad_segment *segs, int nseg, double max_norm, void *scratch, float *out,
+                            hipStream_t s);
+
+// keep_rows.hip
+size_t select_rows_scratch_bytes(int P);
+hipError_t launch_select_rows(const float *score, const uint8_t *protect, int P, int budget, int64_t *rows,
+                              void *scratch, hipStream_t s);
+hipError_t launch_take_rows(const gsr_rows_segment *segs, int nseg, int64_t P, const int64_t *rows, int64_t K,
+                            hipStream_t s);
+
 // knn.hip
 size_t knn_scratch_bytes(int P);
 hipError_t launch_knn(int P, const float *pts, float *dist2, void *scratch, uint32_t *pinned6, hipStream_t s);

@@ -60,6 +60,8 @@ EXPORTED = (
     "gsr_geom_layout", "gsr_binning_layout", "gsr_img_layout", "gsr_last_error", "gsr_abi_version",
     "gsr_timing_enable", "gsr_timing_read", "gsr_stage_name",
     "gsr_l1_ssim_scratch_bytes", "gsr_l1_ssim", "gsr_adam_step", "gsr_densify_stats",
+    "gsr_adamw_step", "gsr_grad_norm_scratch_bytes", "gsr_grad_norm", "gsr_select_rows_scratch_bytes", "gsr_select_rows",
+    "gsr_take_rows",
     "gsr_knn_scratch_bytes", "gsr_knn_mean_dist2",
     "gsr_backward_colors", "gsr_sh_record_floats", "gsr_sh_grad_from_colors", "gsr_backward_planar",
     "gsr_backward_colors_render", "gsr_backward_colors_finish", "gsr_point_list_keys", "gsr_backward_leaves",
@@ -226,6 +228,28 @@ class GsrAdamSegment(ctypes.Structure):
 
 
 ADAM_MAX_SEGS = 8
+
+
+class GsrAdamWSegment(ctypes.Structure):
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("exp_avg", ctypes.c_void_p),
+                ("exp_second", ctypes.c_void_p), ("avg_scale", ctypes.c_void_p), ("second_scale", ctypes.c_void_p),
+                ("n", ctypes.c_int64), ("lr", ctypes.c_double), ("weight_decay", ctypes.c_double),
+                ("step", ctypes.c_int32), ("ordinal", ctypes.c_int32)]
+
+
+class GsrGradSegment(ctypes.Structure):
+    _fields_ = [("grad", ctypes.c_void_p), ("n", ctypes.c_int64), ("dtype", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
+class GsrRowsSegment(ctypes.Structure):
+    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("src_scale", ctypes.c_void_p),
+                ("dst_scale", ctypes.c_void_p), ("row_bytes", ctypes.c_int64), ("kind", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1}  # gsr.h GSR_DTYPE_*
+ROWS_PLAIN, ROWS_E4M3, ROWS_E4M3_SIGNED = 0, 1, 2
 ABI_VERSION = 12
 
 _lib = None
@@ -322,6 +346,19 @@ def load_library():
     lib.gsr_adam_step.restype = ctypes.c_int
     lib.gsr_densify_stats.argtypes = [i32, vp, vp, i32, vp, vp, vp, vp]
     lib.gsr_densify_stats.restype = ctypes.c_int
+    lib.gsr_adamw_step.argtypes = [ctypes.POINTER(GsrAdamWSegment), i32, i32, i32, ctypes.c_double, ctypes.c_double,
+                                   ctypes.c_double, vp, ctypes.c_uint64, vp]
+    lib.gsr_adamw_step.restype = ctypes.c_int
+    lib.gsr_grad_norm_scratch_bytes.argtypes = [i32]
+    lib.gsr_grad_norm_scratch_bytes.restype = sz
+    lib.gsr_grad_norm.argtypes = [ctypes.POINTER(GsrGradSegment), i32, ctypes.c_double, vp, vp, vp]
+    lib.gsr_grad_norm.restype = ctypes.c_int
+    lib.gsr_select_rows_scratch_bytes.argtypes = [i32]
+    lib.gsr_select_rows_scratch_bytes.restype = sz
+    lib.gsr_select_rows.argtypes = [vp, vp, i32, i32, vp, vp, vp]
+    lib.gsr_select_rows.restype = ctypes.c_int
+    lib.gsr_take_rows.argtypes = [ctypes.POINTER(GsrRowsSegment), i32, i64, vp, i64, vp]
+    lib.gsr_take_rows.restype = ctypes.c_int
     lib.gsr_knn_scratch_bytes.argtypes = [i32]
     lib.gsr_knn_scratch_bytes.restype = sz
     lib.gsr_knn_mean_dist2.argtypes = [i32, vp, vp, vp, vp]

@@ -7,18 +7,24 @@
 * ``FusedAdam`` — torch.optim.Adam's update (scene/gaussian_model.py:176-205: six
   groups, lr 0 default, eps 1e-15) in one HIP launch over every parameter; state
   (``exp_avg``, ``exp_avg_sq``, ``step``) kept like torch's.
+* ``FusedAdamW`` — AdamW over any number of tensors, with its moments in 32 bits or in
+  8 (``adamw_state`` / ``adamw_step``), and the gradients clipped by their global norm
+  on the device (``grad_norm``).
+* ``select_rows`` / ``take_rows`` — eviction to a budget by an accumulated weight: the
+  rows that stay, and the rows of parameters and optimiser states gathered in one launch.
 * ``densify_stats`` — train.py:126-127 + scene/gaussian_model.py:565-581
   (``max_radii2D``, ``xyz_gradient_accum``, ``denom``) in one HIP launch.
 * ``dist_knn3`` — ``distCUDA2`` of the simple-knn submodule (scene/gaussian_model.py:
   153-155): mean squared distance to the 3 nearest other
   points, exact, through a uniform-grid HIP search.
 
-All three call libgsr.so through the C ABI (include/gsr.h) on the current HIP
+All call libgsr.so through the C ABI (include/gsr.h) on the current HIP
 stream; there is no CPU path.
 """
 from __future__ import annotations
 
 import ctypes
+import math
 
 import numpy as np
 import torch
@@ -130,6 +136,311 @@ class FusedAdam:
                     p.grad = None
                 elif p.grad is not None:
                     p.grad.zero_()
+
+
+# ------------------------------------------------------------------ AdamW, 32- or 8-bit states
+SCALE_BLOCK = 64  # elements that share a scale in an 8-bit state
+_KEYS = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_scale", "exp_rms", "exp_rms_scale")}
+
+
+def _on(device):
+    """The launches of a call go to ``device``, whichever device is current."""
+    return torch.cuda.device(device)
+
+
+def adamw_state(param: torch.Tensor, state_bits: int = 32) -> dict:
+    """The initial AdamW state of a tensor.  32 bits: ``exp_avg`` and ``exp_avg_sq`` in
+    float32, as torch's.  8 bits: ``exp_avg`` and ``exp_rms`` (the root of exp_avg_sq) as
+    float8_e4m3fn of the parameter's shape, with a float8_e8m0fnu scale for every 64
+    elements of the flattened tensor each (``unpack_state8`` gives their values)."""
+    if state_bits == 32:
+        z = lambda: torch.zeros(param.shape, dtype=torch.float32, device=param.device)  # noqa: E731
+        return {"step": 0, "exp_avg": z(), "exp_avg_sq": z()}
+    if state_bits != 8:
+        raise ValueError(f"adamw_state: state_bits must be 32 or 8 (got {state_bits})")
+    nb = -(-param.numel() // SCALE_BLOCK)
+    st = {"step": 0}
+    for k in ("exp_avg", "exp_rms"):
+        st[k] = torch.zeros(param.shape, dtype=torch.uint8, device=param.device).view(torch.float8_e4m3fn)
+        st[k + "_scale"] = torch.zeros(nb, dtype=torch.uint8, device=param.device).view(torch.float8_e8m0fnu)
+    return st
+
+
+def unpack_state8(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """The float32 values of an 8-bit state (``exp_avg`` with ``exp_avg_scale``, or ``exp_rms``
+    with ``exp_rms_scale``), for inspection: torch operations, on any device."""
+    b = scale.view(torch.uint8).to(torch.int32)
+    s = torch.where(b > 0, b << 23, 0x400000).view(torch.float32).repeat_interleave(SCALE_BLOCK)[:codes.numel()]
+    return (codes.reshape(-1).to(torch.float32) * s).view(codes.shape)
+
+
+def _state_bits(st: dict, p: torch.Tensor, who: str) -> int:
+    bits = 32 if "exp_avg_sq" in st else 8
+    n = p.numel()
+    for k in _KEYS[bits]:
+        t = st.get(k)
+        scale = k.endswith("_scale")
+        want = torch.float32 if bits == 32 else (torch.float8_e8m0fnu if scale else torch.float8_e4m3fn)
+        if t is None or t.dtype is not want or t.numel() != (-(-n // SCALE_BLOCK) if scale else n) or \
+                t.device != p.device or not t.is_contiguous():
+            raise RuntimeError(f"{who}: state {k!r} must be contiguous {want} on {p.device} and fit its "
+                               f"parameter of {tuple(p.shape)}" + ("" if t is None else
+                               f" (got {t.dtype} {tuple(t.shape)} on {t.device})"))
+    return bits
+
+
+def _per_tensor(x, n: int, name: str) -> list:
+    if isinstance(x, (int, float)):
+        return [float(x)] * n
+    if len(x) != n:
+        raise ValueError(f"adamw_step: {len(x)} values of {name} for {n} tensors")
+    return [float(v) for v in x]
+
+
+@torch.no_grad()
+def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), eps: float = 1e-15,
+               grad_scale: torch.Tensor = None, seed: int = 0):
+    """One AdamW step in place over lists of tensors: parameters, their gradients and their
+    states (``adamw_state``; 32- and 8-bit ones may be mixed), in one launch for up to 40
+    tensors of a dtype and state width.
+
+    ``lr`` and ``weight_decay``: a number, or one per tensor.  Each state's ``step`` counts
+    its own tensor's steps and is advanced by one.  ``grad_scale``: a float32 scalar on the
+    device that every gradient is multiplied by (``grad_norm``'s second result).  Parameters
+    are float32 or bfloat16, gradients of the same dtype, all contiguous and on one device.
+    8-bit states and bfloat16 parameters are rounded stochastically, by a pure function of
+    ``seed`` (an int of up to 64 bits), the tensor's step, its place in the list and the
+    element: the same call gives the same bits.  Step counts, rates and seed are host values
+    and would be frozen in a captured graph: under capture this raises.
+
+    Everything is validated before any state is advanced."""
+    lib = _C.load_library()
+    n = len(params)
+    if len(grads) != n or len(states) != n:
+        raise ValueError(f"adamw_step: {n} parameters, {len(grads)} gradients, {len(states)} states")
+    lrs, wds = _per_tensor(lr, n, "lr"), _per_tensor(weight_decay, n, "weight_decay")
+    if not n:
+        return
+    dev = params[0].device
+    launches, seen = {}, set()
+    for k in range(n):
+        p, g, st = params[k], grads[k], states[k]
+        if not p.is_cuda:
+            raise RuntimeError("adamw_step: tensors must be on the GPU (no CPU implementation)")
+        dt = _C.DTYPES.get(p.dtype)
+        if dt is None or g.dtype is not p.dtype:
+            raise RuntimeError(f"adamw_step: float32 or bfloat16 parameters with gradients of the same dtype "
+                               f"expected, got {p.dtype} and {g.dtype}")
+        if p.device != dev or g.device != dev:
+            raise RuntimeError(f"adamw_step: tensors on {p.device} and {g.device}, expected {dev}")
+        if g.shape != p.shape:
+            raise RuntimeError(f"adamw_step: gradient {tuple(g.shape)} of a parameter {tuple(p.shape)}")
+        if not (p.is_contiguous() and g.is_contiguous()):
+            raise RuntimeError("adamw_step: parameters and gradients must be contiguous")
+        bits = _state_bits(st, p, "adamw_step")
+        size = p.numel()
+        if not size:
+            continue
+        at = p.data_ptr()
+        if at in seen:
+            raise RuntimeError("adamw_step: a parameter appears twice")
+        seen.add(at)
+        if bits == 32:
+            q = (at, g.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), None, None)
+        else:
+            q = (at, g.data_ptr(), st["exp_avg"].data_ptr(), st["exp_rms"].data_ptr(),
+                 st["exp_avg_scale"].data_ptr(), st["exp_rms_scale"].data_ptr())
+        launches.setdefault((dt, bits), []).append((*q, size, lrs[k], wds[k], st["step"] + 1, k))
+    if grad_scale is not None and (grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1 or
+                                   grad_scale.device != dev):
+        raise RuntimeError(f"adamw_step: grad_scale must be a float32 scalar on {dev}")
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("adamw_step: step counts and rates are host values; not for graph capture")
+    with _on(dev):
+        for (dt, bits), segs in launches.items():
+            table = (_C.GsrAdamWSegment * len(segs))(*segs)
+            _C._check(lib.gsr_adamw_step(table, len(segs), dt, bits, betas[0], betas[1], eps,
+                                         None if grad_scale is None else grad_scale.data_ptr(),
+                                         seed & 0xFFFFFFFFFFFFFFFF, _C._stream(dev)), "gsr_adamw_step")
+    for st in states:
+        st["step"] += 1
+    torch.autograd.graph.increment_version(params)
+
+
+@torch.no_grad()
+def grad_norm(grads, max_norm: float = math.inf):
+    """(norm, scale), two float32 scalars on the device: the 2-norm over all the tensors
+    (float32 or bfloat16; squares and sums in 64 bits), and ``min(1, max_norm / (norm +
+    1e-6))``, torch.nn.utils.clip_grad_norm_'s coefficient, which ``adamw_step`` takes as
+    ``grad_scale``.  The gradients are not written and the host does not wait."""
+    lib = _C.load_library()
+    if not len(grads):
+        raise ValueError("grad_norm: no gradients")
+    dev = grads[0].device
+    segs = []
+    for g in grads:
+        if not g.is_cuda:
+            raise RuntimeError("grad_norm: tensors must be on the GPU (no CPU implementation)")
+        dt = _C.DTYPES.get(g.dtype)
+        if dt is None:
+            raise RuntimeError(f"grad_norm: float32 or bfloat16 expected, got {g.dtype}")
+        if g.device != dev or not g.is_contiguous():
+            raise RuntimeError(f"grad_norm: gradients must be contiguous and on one device ({dev})")
+        segs.append((g.data_ptr(), g.numel(), dt, 0))
+    with _on(dev):
+        out = torch.empty(2, dtype=torch.float32, device=dev)
+        scratch = torch.empty(lib.gsr_grad_norm_scratch_bytes(len(segs)), dtype=torch.uint8, device=dev)
+        _C._check(lib.gsr_grad_norm((_C.GsrGradSegment * len(segs))(*segs), len(segs), float(max_norm),
+                                    scratch.data_ptr(), out.data_ptr(), _C._stream(dev)), "gsr_grad_norm")
+    return out.unbind()
+
+
+class FusedAdamW:
+    """AdamW over param groups (``params``, ``lr``, optionally ``weight_decay``, ``name``), with
+    the moments in 32 bits or in 8 (``state_bits``), and gradients clipped to a global norm of
+    ``max_norm`` (None: not clipped).  ``state[p]`` is ``adamw_state``'s dict: with 32 bits the
+    names that code for torch's optimizer expects.  After each step ``grad_norm`` holds the
+    norm before clipping (a device scalar; None without clipping)."""
+
+    def __init__(self, groups, lr: float = 0.0, betas=(0.9, 0.999), eps: float = 1e-15, weight_decay: float = 0.0,
+                 state_bits: int = 32, max_norm: float = None, seed: int = 0):
+        if state_bits not in _KEYS:
+            raise ValueError(f"FusedAdamW: state_bits must be 32 or 8 (got {state_bits})")
+        self.param_groups = [dict(g) for g in groups]
+        for g in self.param_groups:
+            g.setdefault("lr", lr)
+            g.setdefault("weight_decay", weight_decay)
+        self.betas, self.eps, self.state_bits, self.max_norm, self.seed = betas, eps, state_bits, max_norm, seed
+        self.state = {}
+        self.grad_norm = None
+
+    @torch.no_grad()
+    def step(self):
+        todo = [(g, p) for g in self.param_groups for p in g["params"] if p.grad is not None]
+        if not todo:
+            return
+        params = [p for _, p in todo]
+        grads = [p.grad for p in params]
+        states = [self.state[p] if p in self.state else adamw_state(p, self.state_bits) for p in params]
+        scale = norm = None
+        if self.max_norm is not None:
+            norm, scale = grad_norm(grads, self.max_norm)
+        adamw_step(params, grads, states, [g["lr"] for g, _ in todo], [g["weight_decay"] for g, _ in todo],
+                   self.betas, self.eps, scale, self.seed)
+        self.grad_norm = norm
+        self.state.update(zip(params, states))
+
+    zero_grad = FusedAdam.zero_grad
+
+    @torch.no_grad()
+    def take_rows(self, rows: torch.Tensor, fresh: torch.Tensor = None) -> list:
+        """Replaces every parameter by its rows ``rows`` (``take_rows``) and moves its state along;
+        ``fresh`` (bool, one per row): those rows get the initial state (densified Gaussians:
+        the parent's row, no history).  Returns the new parameters in the groups' order; they
+        are leaves, without gradients.  All parameters must have the same number of rows."""
+        params = [p for g in self.param_groups for p in g["params"]]
+        have = [p for p in params if p in self.state]
+        if fresh is None:
+            new, states = take_rows(params, rows, [self.state[p] for p in have])
+        else:
+            new = take_rows(params, rows)
+            _, states = take_rows([], torch.where(fresh, -1, rows), [self.state[p] for p in have])
+        old = dict(zip(params, new))
+        for p, q in old.items():
+            q.requires_grad_(p.requires_grad)
+        self.state = {old[p]: st for p, st in zip(have, states)}
+        for g in self.param_groups:
+            g["params"] = [old[p] for p in g["params"]]
+        return new
+
+
+# ------------------------------------------------------------------ eviction to a budget
+@torch.no_grad()
+def select_rows(score: torch.Tensor, budget: int, protect: torch.Tensor = None) -> torch.Tensor:
+    """The rows that stay when a model is evicted to ``budget`` rows by an accumulated weight:
+    the indices (int64, ascending) of the min(budget, P) largest of ``score`` ([P] or [P,1],
+    float32).  Of equal scores the lowest index stays; NaN is below every number; rows with
+    ``protect`` (bool, P of them) stay before all others.  The host does not wait."""
+    lib = _C.load_library()
+    _cuda(score, "select_rows")
+    P = score.numel()
+    if score.dim() not in (1, 2) or score.shape[0] != P:
+        raise RuntimeError(f"select_rows: score must be [P] or [P,1], got {tuple(score.shape)}")
+    if isinstance(budget, bool) or not isinstance(budget, int) or budget < 0:
+        raise ValueError(f"select_rows: budget must be an int >= 0 (got {budget!r})")
+    if P >= 1 << 31:
+        raise RuntimeError(f"select_rows: at most 2^31 - 1 rows (got {P})")
+    if protect is not None and (protect.dtype is not torch.bool or protect.numel() != P or
+                                protect.device != score.device):
+        raise RuntimeError(f"select_rows: protect must be {P} bools on {score.device}, got {protect.dtype} "
+                           f"{tuple(protect.shape)} on {protect.device}")
+    dev = score.device
+    with _on(dev):
+        s = score.contiguous()
+        pr = None if protect is None else protect.contiguous()
+        rows = torch.empty(min(budget, P), dtype=torch.int64, device=dev)
+        if rows.numel():
+            scratch = torch.empty(lib.gsr_select_rows_scratch_bytes(P), dtype=torch.uint8, device=dev)
+            _C._check(lib.gsr_select_rows(s.data_ptr(), None if pr is None else pr.data_ptr(), P, rows.numel(),
+                                          rows.data_ptr(), scratch.data_ptr(), _C._stream(dev)), "gsr_select_rows")
+    return rows
+
+
+@torch.no_grad()
+def take_rows(tensors, rows: torch.Tensor, states=None):
+    """``[t[rows] for t in tensors]`` in one launch for up to 48 tensors of any dtype, as new
+    tensors without gradient history.  ``rows``: int64 [K], any order, repeats allowed; an index
+    outside [0, P) gives a row of zeros (-1: a fresh row).  With ``states`` (AdamW state dicts of
+    tensors with P rows, ``adamw_state``) returns (tensors, states): the states' rows, with
+    ``step`` kept; 8-bit values are re-blocked under new scales, which changes a value only
+    where it is below 2^-13 of its new block's largest."""
+    lib = _C.load_library()
+    flat = list(tensors) + [t for st in states or () for k, t in st.items() if k in ("exp_avg", "exp_avg_sq", "exp_rms")]
+    if rows.dtype is not torch.int64 or rows.dim() != 1 or not rows.is_cuda:
+        raise RuntimeError(f"take_rows: rows must be an int64 vector on the GPU, got {rows.dtype} {tuple(rows.shape)} "
+                           f"on {rows.device}")
+    dev, K = rows.device, rows.numel()
+    P = flat[0].shape[0] if flat and flat[0].dim() else 0
+    for t in flat:
+        if t.device != dev or not t.dim() or t.shape[0] != P:
+            raise RuntimeError(f"take_rows: tensors must have the same number of rows and be on {dev}, got "
+                               f"{tuple(t.shape)} on {t.device} beside {P} rows")
+    if K >= 1 << 31:
+        raise RuntimeError(f"take_rows: at most 2^31 - 1 rows (got {K})")
+    bits = [_state_bits(st, st["exp_avg"], "take_rows") for st in states or ()]
+    segs, keep = [], []
+
+    def plain(t):
+        t = t.contiguous()
+        keep.append(t)
+        new = torch.empty((K, *t.shape[1:]), dtype=t.dtype, device=dev)
+        segs.append((t.data_ptr(), new.data_ptr(), None, None, math.prod(t.shape[1:]) * t.element_size(),
+                     _C.ROWS_PLAIN, 0))
+        return new
+
+    def coded(codes, scale, kind):
+        row = math.prod(codes.shape[1:])
+        new = torch.empty((K, *codes.shape[1:]), dtype=codes.dtype, device=dev)
+        sc = torch.empty(-(-K * row // SCALE_BLOCK), dtype=scale.dtype, device=dev)
+        segs.append((codes.data_ptr(), new.data_ptr(), scale.data_ptr(), sc.data_ptr(), row, kind, 0))
+        return new, sc
+
+    with _on(dev):
+        rows = rows.contiguous()
+        out = [plain(t) for t in tensors]
+        new_states = []
+        for st, b in zip(states or (), bits):
+            got = {"step": st["step"]}
+            if b == 32:
+                got["exp_avg"], got["exp_avg_sq"] = plain(st["exp_avg"]), plain(st["exp_avg_sq"])
+            else:
+                for k, kind in (("exp_avg", _C.ROWS_E4M3_SIGNED), ("exp_rms", _C.ROWS_E4M3)):
+                    got[k], got[k + "_scale"] = coded(st[k], st[k + "_scale"], kind)
+            new_states.append(got)
+        if K and segs:
+            _C._check(lib.gsr_take_rows((_C.GsrRowsSegment * len(segs))(*segs), len(segs), P, rows.data_ptr(), K,
+                                        _C._stream(dev)), "gsr_take_rows")
+    return out if states is None else (out, new_states)
 
 
 @torch.no_grad()

@@ -311,9 +311,12 @@ class TrainState:
     """The optimizer side of GaussianModel for a SynthGaussians: the six Adam groups
     (scene/gaussian_model.py:176-205, lr 0 default, eps 1e-15), the xyz learning-rate
     schedule and the densification statistics (:565-581).  ``fused`` swaps torch's
-    Adam and statistics for the HIP kernels of train_ops.py."""
+    Adam and statistics for the HIP kernels of train_ops.py; with it, any of
+    ``state_bits`` (32 or 8: the moments' width), ``weight_decay`` and ``max_norm`` (global
+    gradient norm to clip to) takes train_ops.FusedAdamW instead of FusedAdam."""
 
-    def __init__(self, g, spatial_lr_scale: float, fused: bool = False, opt: dict = OPT):
+    def __init__(self, g, spatial_lr_scale: float, fused: bool = False, opt: dict = OPT, state_bits: int = None,
+                 weight_decay: float = 0.0, max_norm: float = None):
         import train_ops
 
         self.opt, self.fused = opt, fused
@@ -325,7 +328,13 @@ class TrainState:
             {"params": [g.scaling], "lr": opt["scaling_lr"], "name": "scaling"},
             {"params": [g.rotation], "lr": opt["rotation_lr"], "name": "rotation"},
         ]
-        if fused:
+        adamw = state_bits is not None or weight_decay or max_norm is not None
+        if adamw and not fused:
+            raise ValueError("TrainState: state_bits, weight_decay and max_norm need fused=True")
+        if adamw:
+            self.optimizer = train_ops.FusedAdamW(groups, lr=0.0, eps=1e-15, weight_decay=weight_decay,
+                                                  state_bits=state_bits or 32, max_norm=max_norm)
+        elif fused:
             self.optimizer = train_ops.FusedAdam(groups, lr=0.0, eps=1e-15)
         else:
             self.optimizer = torch.optim.Adam(groups, lr=0.0, eps=1e-15)
@@ -343,6 +352,25 @@ class TrainState:
             if group["name"] == "xyz":
                 group["lr"] = self.xyz_scheduler(iteration)
                 return group["lr"]
+
+    @torch.no_grad()
+    def prune_to_budget(self, g, score: torch.Tensor, budget: int, protect: torch.Tensor = None) -> torch.Tensor:
+        """Evicts the Gaussians of the smallest ``score`` ([P]: accumulate_blend_weight over
+        the views) so that ``budget`` stay (train_ops.select_rows: ties, NaN, ``protect``): the
+        model's six parameters, their optimiser states and the densification statistics are
+        replaced by the kept rows, in order.  Returns those rows (int64); the caller's own
+        per-Gaussian tensors follow with train_ops.take_rows.  Needs FusedAdamW."""
+        import train_ops
+
+        if not isinstance(self.optimizer, train_ops.FusedAdamW):
+            raise RuntimeError("prune_to_budget: needs a TrainState with FusedAdamW (state_bits=)")
+        if score.shape[0] != g.xyz.shape[0]:
+            raise RuntimeError(f"prune_to_budget: {score.shape[0]} scores for {g.xyz.shape[0]} Gaussians")
+        rows = train_ops.select_rows(score, budget, protect)
+        (g.xyz, g.features_dc, g.features_rest, g.opacity, g.scaling, g.rotation) = self.optimizer.take_rows(rows)
+        self.xyz_gradient_accum, self.denom, self.max_radii2D = train_ops.take_rows(
+            [self.xyz_gradient_accum, self.denom, self.max_radii2D], rows)
+        return rows
 
     def reduce_densification_stats(self, group=None):
         """View-parallel: the per-rank statistics SUM / SUM / MAX-reduced over the group
@@ -363,6 +391,23 @@ class TrainState:
             self.max_radii2D[vis] = torch.max(self.max_radii2D[vis], radii[vis])
             self.xyz_gradient_accum[vis] += torch.norm(vsp.grad[vis, :2], dim=-1, keepdim=True)
             self.denom[vis] += 1
+
+
+def accumulate_blend_weight(camera, gaussians, bg: torch.Tensor, score: torch.Tensor) -> torch.Tensor:
+    """score[i] += sum over the view's pixels of T_i alpha_i, the weight with which Gaussian
+    i's colour enters the pixel: the gradient of the image's first channel with respect to
+    the Gaussians' (overridden) colours, from the rasterizer's own backward.  ``score``:
+    [P] float32, in place."""
+    if score.shape != (gaussians.xyz.shape[0],) or score.dtype is not torch.float32:
+        raise RuntimeError(f"accumulate_blend_weight: score must be [{gaussians.xyz.shape[0]}] float32, got "
+                           f"{tuple(score.shape)} {score.dtype}")
+    with torch.enable_grad():
+        colours = torch.ones_like(gaussians.xyz).requires_grad_(True)
+        image = render(camera, gaussians, bg, override_color=colours)["render"]
+        seed = torch.zeros_like(image)
+        seed[0] = 1.0
+        (grad,) = torch.autograd.grad(image, colours, seed)
+    return score.add_(grad[:, 0])
 
 
 def full_train_step(iteration: int, camera, gaussians, state: TrainState, target: torch.Tensor,

@@ -503,6 +503,77 @@ typedef struct {
 int gsr_adam_step(const gsr_adam_segment *segs, int32_t nseg, int32_t step, double beta1, double beta2, double eps,
                   void *stream);
 
+/* gsr_adamw_step: AdamW (decoupled weight decay) over any number of tensors:
+ *   g' = c g,  m' = m + (1 - beta1) (g' - m),  v' = beta2 v + (1 - beta2) g'^2,
+ *   p' = p (1 - lr wd) - lr / (1 - beta1^t) m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)
+ * with t = step, the segment's 1-based count after the increment, and c = *grad_scale
+ * (device; NULL = 1; gsr_grad_norm's out + 1).  dtype: of parameters and gradients.
+ * state_bits 32: exp_avg = m, exp_second = v, both float[n]; the scale pointers are
+ * not read.  state_bits 8: exp_avg holds m and exp_second holds sqrt(v) as OCP e4m3
+ * codes, one byte an element; element i has the value code_i 2^(scale[i / 64] - 127),
+ * with ceil(n / 64) scale bytes; a state of all zero bytes is the initial one.  Codes
+ * and bf16 parameters are rounded stochastically, from a pure function of (seed, step,
+ * ordinal, element).  A moment that is NaN or 2^127 or more becomes its element's NaN code.
+ * n <= 2^33 per segment.  Segments must not overlap. */
+#define GSR_DTYPE_F32 0
+#define GSR_DTYPE_BF16 1
+typedef struct {
+    void *param;
+    const void *grad;
+    void *exp_avg;
+    void *exp_second;
+    uint8_t *avg_scale;
+    uint8_t *second_scale;
+    int64_t n;
+    double lr;
+    double weight_decay;
+    int32_t step;
+    int32_t ordinal; /* the tensor's place in the caller's list */
+} gsr_adamw_segment;
+int gsr_adamw_step(const gsr_adamw_segment *segs, int32_t nseg, int32_t dtype, int32_t state_bits, double beta1,
+                   double beta2, double eps, const float *grad_scale, uint64_t seed, void *stream);
+
+/* gsr_grad_norm: out[0] = the 2-norm over all segments (summed in 64 bits), out[1] =
+ * min(1, max_norm / (norm + 1e-6)), both float on the device; no host wait.
+ * scratch: gsr_grad_norm_scratch_bytes(nseg). */
+typedef struct {
+    const void *grad;
+    int64_t n;
+    int32_t dtype;
+    int32_t reserved;
+} gsr_grad_segment;
+size_t gsr_grad_norm_scratch_bytes(int32_t nseg);
+int gsr_grad_norm(const gsr_grad_segment *segs, int32_t nseg, double max_norm, void *scratch, float *out,
+                  void *stream);
+
+/* gsr_select_rows: the indices of the `budget` largest of score[P], ascending, into
+ * rows[min(budget, P)].  Equal scores: the lowest index stays.  -0 equals +0, NaN is
+ * below every number, protect[i] != 0 (NULL: none) above every one.  No host wait.
+ * scratch: gsr_select_rows_scratch_bytes(P). */
+size_t gsr_select_rows_scratch_bytes(int32_t P);
+int gsr_select_rows(const float *score, const uint8_t *protect, int32_t P, int32_t budget, int64_t *rows,
+                    void *scratch, void *stream);
+
+/* gsr_take_rows: dst[j] = src[rows[j]], j in [0, K), for every segment; zeros where
+ * rows[j] is outside [0, P).  Plain segments: rows of row_bytes bytes.  E4M3 segments
+ * (gsr_adamw_step's 8-bit states): row_bytes codes a row, whose values are given codes
+ * and scales for the blocks that they land in (to nearest even; the magnitudes of
+ * GSR_ROWS_E4M3, sqrt(v), never go from nonzero to zero).  dst must not overlap src. */
+#define GSR_ROWS_PLAIN 0
+#define GSR_ROWS_E4M3 1
+#define GSR_ROWS_E4M3_SIGNED 2
+typedef struct {
+    const void *src;
+    void *dst;
+    const uint8_t *src_scale;
+    uint8_t *dst_scale;
+    int64_t row_bytes;
+    int32_t kind;
+    int32_t reserved;
+} gsr_rows_segment;
+int gsr_take_rows(const gsr_rows_segment *segs, int32_t nseg, int64_t P, const int64_t *rows, int64_t K,
+                  void *stream);
+
 /* gsr_densify_stats: for radii[i] > 0: max_radii2D[i] = max(max_radii2D[i], radii[i]),
  * xyz_gradient_accum[i] += |viewspace_grad[i, 0:2]|, denom[i] += 1
  * (train.py:126-127, scene/gaussian_model.py:565-581).  viewspace_grad rows
