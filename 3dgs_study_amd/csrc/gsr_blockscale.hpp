@@ -64,21 +64,14 @@ __device__ __forceinline__ uint32_t e4m3_round(float x, uint32_t u, uint32_t rou
     c = a < E4M3_TOP ? c : 0x7Fu;
     return SIGNED ? c | ((bits >> 24) & 0x80u) : c;
 }
-__device__ __forceinline__ uint32_t e4m3_units(float x, uint32_t byte, int exp = 0) {
-    return as_u32(__builtin_ldexpf(as_f32(coded_bits(x)), 7 + exp - (int)byte));
+__device__ __forceinline__ uint32_t e4m3_units(float x, uint32_t byte) {
+    return as_u32(__builtin_ldexpf(as_f32(coded_bits(x)), 7 - (int)byte));
 }
 // dither: 16 random bits, centred in the 20 that are dropped
 template <bool SIGNED>
 __device__ __forceinline__ uint32_t e4m3_stochastic(float x, uint32_t byte, uint32_t dither) {
     return e4m3_round<SIGNED>(x, e4m3_units(x, byte), dither << 4 | 8u);
 }
-// x is given in units of 2^exp
-template <bool SIGNED>
-__device__ __forceinline__ uint32_t e4m3_nearest(float x, uint32_t byte, int exp) {
-    const uint32_t u = e4m3_units(x, byte, exp);
-    return e4m3_round<SIGNED>(x, u, 0x7FFFFu + ((u >> 20) & 1u));
-}
-
 // A 32-bit mixing (xor-shifts and odd multipliers: the fractional bits of the roots of
 // 2 and 3), and the random word of element i of a tensor from the tensor's key: a pure
 // function, so a run repeats and every replica of a data-parallel job rounds alike.
@@ -101,5 +94,6 @@ __device__ __forceinline__ uint32_t dither_word(uint64_t i, uint32_t key) {
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint16_t u16x4_u __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32_u __attribute__((aligned(1)));
+typedef uint16_t u16_u __attribute__((aligned(1)));
 
 }  // namespace gsr
