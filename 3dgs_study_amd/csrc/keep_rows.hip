@@ -184,6 +184,56 @@ __global__ void __launch_bounds__(SR_THREADS) select_write_kernel(SelectArgs a) 
     }
 }
 
+// Up to SR_SMALL scores: one workgroup, the keys in registers (SR_PER consecutive ones a
+// thread), the histograms in LDS: one launch instead of six.
+constexpr int SR_PER = 16, SR_SMALL = SR_HIST_THREADS * SR_PER;
+__global__ void __launch_bounds__(SR_HIST_THREADS) select_small_kernel(SelectArgs a) {
+    __shared__ uint32_t h[SR_BINS * SR_COPIES], total[SR_BINS], sh[32];
+    const int64_t i0 = (int64_t)threadIdx.x * SR_PER;
+    const uint32_t copy = threadIdx.x % SR_COPIES;
+    uint32_t key[SR_PER], prefix = 0, keep = a.budget;
+    int live = 0;
+#pragma unroll
+    for (int j = 0; j < SR_PER; j += 4) live += score_keys(a, i0 + j, key + j);
+#pragma unroll
+    for (int d = 0; d < 3; d++) {
+        const int shift = d == 0 ? 21 : (d == 1 ? 10 : 0), bits = d == 2 ? 10 : 11;
+        for (int i = threadIdx.x; i < SR_BINS * SR_COPIES; i += SR_HIST_THREADS) h[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < SR_PER; j++)
+            if (j < live && (d == 0 || key[j] >> (shift + bits) == prefix))
+                atomicAdd(&h[(key[j] >> shift & ((1u << bits) - 1)) * SR_COPIES + copy], 1u);
+        __syncthreads();
+        for (int i = threadIdx.x; i < SR_BINS; i += SR_HIST_THREADS) {
+            uint32_t n = 0;
+#pragma unroll
+            for (int c = 0; c < SR_COPIES; c++) n += h[i * SR_COPIES + c];
+            total[i] = n;
+        }
+        __syncthreads();
+        uint32_t bin, rest;
+        resolve_digit<SR_HIST_THREADS>(total, keep, sh, &bin, &rest);
+        prefix = prefix << bits | bin;
+        keep = rest;
+    }
+    uint32_t own = 0, tot;
+#pragma unroll
+    for (int j = 0; j < SR_PER; j++)
+        if (j < live) own += key[j] > prefix ? 1u : (key[j] == prefix ? 0x10000u : 0u);  // <= 16384 each
+    const uint32_t before = block_inclusive_scan<SR_HIST_THREADS>(own, sh, &tot) - own;
+    uint32_t g = before & 0xFFFFu, e = before >> 16;
+#pragma unroll
+    for (int j = 0; j < SR_PER; j++) {
+        if (j >= live) continue;
+        if (key[j] > prefix) a.rows[g++ + min(e, keep)] = i0 + j;
+        else if (key[j] == prefix) {
+            if (e < keep) a.rows[g + e] = i0 + j;
+            e++;
+        }
+    }
+}
+
 size_t select_rows_scratch_bytes(int P) {
     return (3 * SR_BINS + 16 + 2 * (((size_t)P + SR_TILE - 1) / SR_TILE)) * 4;
 }
@@ -193,6 +243,10 @@ hipError_t launch_select_rows(const float *score, const uint8_t *protect, int P,
     SelectArgs a;
     a.score = score, a.protect = protect, a.rows = rows;
     a.P = P, a.budget = (uint32_t)budget;
+    if (P <= SR_SMALL) {
+        hipLaunchKernelGGL(select_small_kernel, dim3(1), dim3(SR_HIST_THREADS), 0, st, a);
+        return hipGetLastError();
+    }
     a.tiles = (int)(((int64_t)P + SR_TILE - 1) / SR_TILE);
     a.hist = (uint32_t *)scratch;
     a.ctrl = a.hist + 3 * SR_BINS;

@@ -346,18 +346,19 @@ def load_library():
     lib.gsr_adam_step.restype = ctypes.c_int
     lib.gsr_densify_stats.argtypes = [i32, vp, vp, i32, vp, vp, vp, vp]
     lib.gsr_densify_stats.restype = ctypes.c_int
-    lib.gsr_adamw_step.argtypes = [ctypes.POINTER(GsrAdamWSegment), i32, i32, i32, ctypes.c_double, ctypes.c_double,
+    lib.gsr_adamw_step.argtypes = [vp, i32,  # gsr_adamw_segment[]: a structure array or packed bytes
+                                   i32, i32, ctypes.c_double, ctypes.c_double,
                                    ctypes.c_double, vp, ctypes.c_uint64, vp]
     lib.gsr_adamw_step.restype = ctypes.c_int
     lib.gsr_grad_norm_scratch_bytes.argtypes = [i32]
     lib.gsr_grad_norm_scratch_bytes.restype = sz
-    lib.gsr_grad_norm.argtypes = [ctypes.POINTER(GsrGradSegment), i32, ctypes.c_double, vp, vp, vp]
+    lib.gsr_grad_norm.argtypes = [vp, i32, ctypes.c_double, vp, vp, vp]
     lib.gsr_grad_norm.restype = ctypes.c_int
     lib.gsr_select_rows_scratch_bytes.argtypes = [i32]
     lib.gsr_select_rows_scratch_bytes.restype = sz
     lib.gsr_select_rows.argtypes = [vp, vp, i32, i32, vp, vp, vp]
     lib.gsr_select_rows.restype = ctypes.c_int
-    lib.gsr_take_rows.argtypes = [ctypes.POINTER(GsrRowsSegment), i32, i64, vp, i64, vp]
+    lib.gsr_take_rows.argtypes = [vp, i32, i64, vp, i64, vp]
     lib.gsr_take_rows.restype = ctypes.c_int
     lib.gsr_knn_scratch_bytes.argtypes = [i32]
     lib.gsr_knn_scratch_bytes.restype = sz

@@ -23,8 +23,10 @@ stream; there is no CPU path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
+import struct
 
 import numpy as np
 import torch
@@ -143,9 +145,12 @@ SCALE_BLOCK = 64  # elements that share a scale in an 8-bit state
 _KEYS = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_scale", "exp_rms", "exp_rms_scale")}
 
 
+_SAME = contextlib.nullcontext()
+
+
 def _on(device):
     """The launches of a call go to ``device``, whichever device is current."""
-    return torch.cuda.device(device)
+    return _SAME if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def adamw_state(param: torch.Tensor, state_bits: int = 32) -> dict:
@@ -174,7 +179,7 @@ def unpack_state8(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     return (codes.reshape(-1).to(torch.float32) * s).view(codes.shape)
 
 
-def _state_bits(st: dict, p: torch.Tensor, who: str) -> int:
+def _state_refuse(st: dict, p: torch.Tensor, who: str):
     bits = 32 if "exp_avg_sq" in st else 8
     n = p.numel()
     for k in _KEYS[bits]:
@@ -186,7 +191,26 @@ def _state_bits(st: dict, p: torch.Tensor, who: str) -> int:
             raise RuntimeError(f"{who}: state {k!r} must be contiguous {want} on {p.device} and fit its "
                                f"parameter of {tuple(p.shape)}" + ("" if t is None else
                                f" (got {t.dtype} {tuple(t.shape)} on {t.device})"))
-    return bits
+
+
+def _state_ptrs(st: dict, p: torch.Tensor, n: int, who: str) -> tuple:
+    """(bits, then exp_avg, exp_second and their scales' addresses) of a checked state of ``p``."""
+    at = p.get_device()
+    v = st.get("exp_avg_sq")
+    m = st.get("exp_avg")
+    if v is not None:
+        if m is None or not (m.dtype is v.dtype is torch.float32 and m.numel() == n == v.numel() and
+                             m.get_device() == at == v.get_device() and m.is_contiguous() and v.is_contiguous()):
+            _state_refuse(st, p, who)
+        return 32, m.data_ptr(), v.data_ptr(), 0, 0
+    r, ms, rs = st.get("exp_rms"), st.get("exp_avg_scale"), st.get("exp_rms_scale")
+    if m is None or r is None or ms is None or rs is None or not (
+            m.dtype is r.dtype is torch.float8_e4m3fn and ms.dtype is rs.dtype is torch.float8_e8m0fnu and
+            m.numel() == n == r.numel() and ms.numel() == rs.numel() == -(-n // SCALE_BLOCK) and
+            m.get_device() == r.get_device() == ms.get_device() == rs.get_device() == at and
+            m.is_contiguous() and r.is_contiguous() and ms.is_contiguous() and rs.is_contiguous()):
+        _state_refuse(st, p, who)
+    return 8, m.data_ptr(), r.data_ptr(), ms.data_ptr(), rs.data_ptr()
 
 
 def _per_tensor(x, n: int, name: str) -> list:
@@ -197,7 +221,19 @@ def _per_tensor(x, n: int, name: str) -> list:
     return [float(v) for v in x]
 
 
-@torch.no_grad()
+def _adamw_refuse(p: torch.Tensor, g: torch.Tensor, dev):
+    if not p.is_cuda:
+        raise RuntimeError("adamw_step: tensors must be on the GPU (no CPU implementation)")
+    if p.dtype not in _C.DTYPES or g.dtype is not p.dtype:
+        raise RuntimeError(f"adamw_step: float32 or bfloat16 parameters with gradients of the same dtype "
+                           f"expected, got {p.dtype} and {g.dtype}")
+    if p.device != dev or g.device != dev:
+        raise RuntimeError(f"adamw_step: tensors on {p.device} and {g.device}, expected {dev}")
+    if g.shape != p.shape:
+        raise RuntimeError(f"adamw_step: gradient {tuple(g.shape)} of a parameter {tuple(p.shape)}")
+    raise RuntimeError("adamw_step: parameters and gradients must be contiguous")
+
+
 def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), eps: float = 1e-15,
                grad_scale: torch.Tensor = None, seed: int = 0):
     """One AdamW step in place over lists of tensors: parameters, their gradients and their
@@ -221,36 +257,23 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
     lrs, wds = _per_tensor(lr, n, "lr"), _per_tensor(weight_decay, n, "weight_decay")
     if not n:
         return
-    dev = params[0].device
+    dev, at = params[0].device, params[0].get_device()
     launches, seen = {}, set()
-    for k in range(n):
-        p, g, st = params[k], grads[k], states[k]
-        if not p.is_cuda:
-            raise RuntimeError("adamw_step: tensors must be on the GPU (no CPU implementation)")
-        dt = _C.DTYPES.get(p.dtype)
-        if dt is None or g.dtype is not p.dtype:
-            raise RuntimeError(f"adamw_step: float32 or bfloat16 parameters with gradients of the same dtype "
-                               f"expected, got {p.dtype} and {g.dtype}")
-        if p.device != dev or g.device != dev:
-            raise RuntimeError(f"adamw_step: tensors on {p.device} and {g.device}, expected {dev}")
-        if g.shape != p.shape:
-            raise RuntimeError(f"adamw_step: gradient {tuple(g.shape)} of a parameter {tuple(p.shape)}")
-        if not (p.is_contiguous() and g.is_contiguous()):
-            raise RuntimeError("adamw_step: parameters and gradients must be contiguous")
-        bits = _state_bits(st, p, "adamw_step")
+    for k, (p, g, st) in enumerate(zip(params, grads, states)):
+        dt = p.dtype
+        if at < 0 or dt not in _C.DTYPES or g.dtype is not dt or p.get_device() != at or g.get_device() != at or \
+                g.shape != p.shape or not (p.is_contiguous() and g.is_contiguous()):
+            _adamw_refuse(p, g, dev)
         size = p.numel()
+        bits, m, v, ms, vs = _state_ptrs(st, p, size, "adamw_step")
         if not size:
             continue
-        at = p.data_ptr()
-        if at in seen:
+        addr = p.data_ptr()
+        if addr in seen:
             raise RuntimeError("adamw_step: a parameter appears twice")
-        seen.add(at)
-        if bits == 32:
-            q = (at, g.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), None, None)
-        else:
-            q = (at, g.data_ptr(), st["exp_avg"].data_ptr(), st["exp_rms"].data_ptr(),
-                 st["exp_avg_scale"].data_ptr(), st["exp_rms_scale"].data_ptr())
-        launches.setdefault((dt, bits), []).append((*q, size, lrs[k], wds[k], st["step"] + 1, k))
+        seen.add(addr)
+        launches.setdefault((dt, bits), []).extend((addr, g.data_ptr(), m, v, ms, vs, size, lrs[k], wds[k],
+                                                    st["step"] + 1, k))
     if grad_scale is not None and (grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1 or
                                    grad_scale.device != dev):
         raise RuntimeError(f"adamw_step: grad_scale must be a float32 scalar on {dev}")
@@ -258,16 +281,15 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
         raise RuntimeError("adamw_step: step counts and rates are host values; not for graph capture")
     with _on(dev):
         for (dt, bits), segs in launches.items():
-            table = (_C.GsrAdamWSegment * len(segs))(*segs)
-            _C._check(lib.gsr_adamw_step(table, len(segs), dt, bits, betas[0], betas[1], eps,
-                                         None if grad_scale is None else grad_scale.data_ptr(),
+            count = len(segs) // 11  # gsr_adamw_segment's fields
+            _C._check(lib.gsr_adamw_step(struct.pack("7q2d2i" * count, *segs), count, _C.DTYPES[dt], bits, betas[0],
+                                         betas[1], eps, None if grad_scale is None else grad_scale.data_ptr(),
                                          seed & 0xFFFFFFFFFFFFFFFF, _C._stream(dev)), "gsr_adamw_step")
     for st in states:
         st["step"] += 1
     torch.autograd.graph.increment_version(params)
 
 
-@torch.no_grad()
 def grad_norm(grads, max_norm: float = math.inf):
     """(norm, scale), two float32 scalars on the device: the 2-norm over all the tensors
     (float32 or bfloat16; squares and sums in 64 bits), and ``min(1, max_norm / (norm +
@@ -276,22 +298,22 @@ def grad_norm(grads, max_norm: float = math.inf):
     lib = _C.load_library()
     if not len(grads):
         raise ValueError("grad_norm: no gradients")
-    dev = grads[0].device
+    dev, at = grads[0].device, grads[0].get_device()
     segs = []
     for g in grads:
-        if not g.is_cuda:
-            raise RuntimeError("grad_norm: tensors must be on the GPU (no CPU implementation)")
-        dt = _C.DTYPES.get(g.dtype)
-        if dt is None:
-            raise RuntimeError(f"grad_norm: float32 or bfloat16 expected, got {g.dtype}")
-        if g.device != dev or not g.is_contiguous():
+        if g.get_device() != at or at < 0 or g.dtype not in _C.DTYPES or not g.is_contiguous():
+            if not g.is_cuda:
+                raise RuntimeError("grad_norm: tensors must be on the GPU (no CPU implementation)")
+            if g.dtype not in _C.DTYPES:
+                raise RuntimeError(f"grad_norm: float32 or bfloat16 expected, got {g.dtype}")
             raise RuntimeError(f"grad_norm: gradients must be contiguous and on one device ({dev})")
-        segs.append((g.data_ptr(), g.numel(), dt, 0))
+        segs += (g.data_ptr(), g.numel(), _C.DTYPES[g.dtype])
+    count = len(grads)
     with _on(dev):
         out = torch.empty(2, dtype=torch.float32, device=dev)
-        scratch = torch.empty(lib.gsr_grad_norm_scratch_bytes(len(segs)), dtype=torch.uint8, device=dev)
-        _C._check(lib.gsr_grad_norm((_C.GsrGradSegment * len(segs))(*segs), len(segs), float(max_norm),
-                                    scratch.data_ptr(), out.data_ptr(), _C._stream(dev)), "gsr_grad_norm")
+        scratch = torch.empty(lib.gsr_grad_norm_scratch_bytes(count), dtype=torch.uint8, device=dev)
+        _C._check(lib.gsr_grad_norm(struct.pack("3q" * count, *segs), count, float(max_norm), scratch.data_ptr(),
+                                    out.data_ptr(), _C._stream(dev)), "gsr_grad_norm")
     return out.unbind()
 
 
@@ -355,7 +377,6 @@ class FusedAdamW:
 
 
 # ------------------------------------------------------------------ eviction to a budget
-@torch.no_grad()
 def select_rows(score: torch.Tensor, budget: int, protect: torch.Tensor = None) -> torch.Tensor:
     """The rows that stay when a model is evicted to ``budget`` rows by an accumulated weight:
     the indices (int64, ascending) of the min(budget, P) largest of ``score`` ([P] or [P,1],
@@ -386,7 +407,6 @@ def select_rows(score: torch.Tensor, budget: int, protect: torch.Tensor = None) 
     return rows
 
 
-@torch.no_grad()
 def take_rows(tensors, rows: torch.Tensor, states=None):
     """``[t[rows] for t in tensors]`` in one launch for up to 48 tensors of any dtype, as new
     tensors without gradient history.  ``rows``: int64 [K], any order, repeats allowed; an index
@@ -395,50 +415,60 @@ def take_rows(tensors, rows: torch.Tensor, states=None):
     ``step`` kept; 8-bit values are re-blocked under new scales, which changes a value only
     where it is below 2^-13 of its new block's largest."""
     lib = _C.load_library()
-    flat = list(tensors) + [t for st in states or () for k, t in st.items() if k in ("exp_avg", "exp_avg_sq", "exp_rms")]
     if rows.dtype is not torch.int64 or rows.dim() != 1 or not rows.is_cuda:
         raise RuntimeError(f"take_rows: rows must be an int64 vector on the GPU, got {rows.dtype} {tuple(rows.shape)} "
                            f"on {rows.device}")
-    dev, K = rows.device, rows.numel()
-    P = flat[0].shape[0] if flat and flat[0].dim() else 0
-    for t in flat:
-        if t.device != dev or not t.dim() or t.shape[0] != P:
-            raise RuntimeError(f"take_rows: tensors must have the same number of rows and be on {dev}, got "
-                               f"{tuple(t.shape)} on {t.device} beside {P} rows")
+    dev, at, K = rows.device, rows.get_device(), rows.numel()
     if K >= 1 << 31:
         raise RuntimeError(f"take_rows: at most 2^31 - 1 rows (got {K})")
-    bits = [_state_bits(st, st["exp_avg"], "take_rows") for st in states or ()]
+    P = None
     segs, keep = [], []
 
+    def shape_of(t):
+        nonlocal P
+        s = t.shape
+        if t.get_device() != at or not s or s[0] != (s[0] if P is None else P):
+            raise RuntimeError(f"take_rows: tensors must have the same number of rows and be on {dev}, got "
+                               f"{tuple(s)} on {t.device}" + ("" if P is None else f" beside {P} rows"))
+        P = s[0]
+        return s
+
     def plain(t):
-        t = t.contiguous()
-        keep.append(t)
-        new = torch.empty((K, *t.shape[1:]), dtype=t.dtype, device=dev)
-        segs.append((t.data_ptr(), new.data_ptr(), None, None, math.prod(t.shape[1:]) * t.element_size(),
-                     _C.ROWS_PLAIN, 0))
+        s = shape_of(t)
+        if not t.is_contiguous():
+            t = t.contiguous()
+            keep.append(t)  # until the launch
+        new = t.new_empty((K, *s[1:]))
+        segs.extend((t.data_ptr(), new.data_ptr(), 0, 0, t.nbytes // P if P else math.prod(s[1:]) * t.element_size(),
+                     _C.ROWS_PLAIN))
         return new
 
-    def coded(codes, scale, kind):
-        row = math.prod(codes.shape[1:])
-        new = torch.empty((K, *codes.shape[1:]), dtype=codes.dtype, device=dev)
-        sc = torch.empty(-(-K * row // SCALE_BLOCK), dtype=scale.dtype, device=dev)
-        segs.append((codes.data_ptr(), new.data_ptr(), scale.data_ptr(), sc.data_ptr(), row, kind, 0))
+    def coded(codes, src, scale, src_scale, kind):
+        s = shape_of(codes)
+        row = codes.numel() // P if P else math.prod(s[1:])
+        new = codes.new_empty((K, *s[1:]))
+        sc = scale.new_empty(-(-K * row // SCALE_BLOCK))
+        segs.extend((src, new.data_ptr(), src_scale, sc.data_ptr(), row, kind))
         return new, sc
 
     with _on(dev):
-        rows = rows.contiguous()
+        if not rows.is_contiguous():
+            rows = rows.contiguous()
         out = [plain(t) for t in tensors]
         new_states = []
-        for st, b in zip(states or (), bits):
+        for st in states or ():
+            m = st["exp_avg"]
+            bits, mp, vp, msp, vsp = _state_ptrs(st, m, m.numel(), "take_rows")
             got = {"step": st["step"]}
-            if b == 32:
-                got["exp_avg"], got["exp_avg_sq"] = plain(st["exp_avg"]), plain(st["exp_avg_sq"])
+            if bits == 32:
+                got["exp_avg"], got["exp_avg_sq"] = plain(m), plain(st["exp_avg_sq"])
             else:
-                for k, kind in (("exp_avg", _C.ROWS_E4M3_SIGNED), ("exp_rms", _C.ROWS_E4M3)):
-                    got[k], got[k + "_scale"] = coded(st[k], st[k + "_scale"], kind)
+                got["exp_avg"], got["exp_avg_scale"] = coded(m, mp, st["exp_avg_scale"], msp, _C.ROWS_E4M3_SIGNED)
+                got["exp_rms"], got["exp_rms_scale"] = coded(st["exp_rms"], vp, st["exp_rms_scale"], vsp, _C.ROWS_E4M3)
             new_states.append(got)
         if K and segs:
-            _C._check(lib.gsr_take_rows((_C.GsrRowsSegment * len(segs))(*segs), len(segs), P, rows.data_ptr(), K,
+            count = len(segs) // 6  # gsr_rows_segment's fields, the last two as one
+            _C._check(lib.gsr_take_rows(struct.pack(f"{6 * count}q", *segs), count, P, rows.data_ptr(), K,
                                         _C._stream(dev)), "gsr_take_rows")
     return out if states is None else (out, new_states)
 
