@@ -54,21 +54,23 @@ struct Elems;
 template <>
 struct Elems<float> {
     static __device__ __forceinline__ void load4(const float *s, float x[4]) {
-        const f32x4_u v = *reinterpret_cast<const f32x4_u *>(s);
+        const f32x4_u *at = reinterpret_cast<const f32x4_u *>(s);
+        const f32x4_u v = __builtin_nontemporal_load(at);
         x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
     }
     static __device__ __forceinline__ float load(const float *s) { return *s; }
     static __device__ __forceinline__ float round(float x, uint32_t) { return x; }
     static __device__ __forceinline__ void store4(float *d, const float x[4]) {
-        f32x4_u v = {x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<f32x4_u *>(d) = v;
+        f32x4_u v = {x[0], x[1], x[2], x[3]}, *at = reinterpret_cast<f32x4_u *>(d);
+        __builtin_nontemporal_store(v, at);
     }
     static __device__ __forceinline__ void store(float *d, float x) { *d = x; }
 };
 template <>
 struct Elems<uint16_t> {  // bf16
     static __device__ __forceinline__ void load4(const uint16_t *s, float x[4]) {
-        const u16x4_u v = *reinterpret_cast<const u16x4_u *>(s);
+        const u16x4_u *at = reinterpret_cast<const u16x4_u *>(s);
+        const u16x4_u v = __builtin_nontemporal_load(at);
         x[0] = as_f32((uint32_t)v.x << 16), x[1] = as_f32((uint32_t)v.y << 16);
         x[2] = as_f32((uint32_t)v.z << 16), x[3] = as_f32((uint32_t)v.w << 16);
     }
@@ -82,7 +84,8 @@ struct Elems<uint16_t> {  // bf16
     static __device__ __forceinline__ void store4(uint16_t *d, const float x[4]) {
         u16x4_u v = {(uint16_t)(as_u32(x[0]) >> 16), (uint16_t)(as_u32(x[1]) >> 16), (uint16_t)(as_u32(x[2]) >> 16),
                      (uint16_t)(as_u32(x[3]) >> 16)};
-        *reinterpret_cast<u16x4_u *>(d) = v;
+        u16x4_u *at = reinterpret_cast<u16x4_u *>(d);
+        __builtin_nontemporal_store(v, at);
     }
     static __device__ __forceinline__ void store(uint16_t *d, float x) { *d = (uint16_t)(as_u32(x) >> 16); }
 };
@@ -107,86 +110,119 @@ __device__ __forceinline__ void adamw_one(const AdamWArgs &a, const AdamWSeg &s,
     p = p * s.decay + (m / (r * s.inv_bc2 + a.eps)) * s.neg_step;
 }
 
+// Four consecutive elements of a segment, as a lane holds them
+template <typename T, bool BITS8>
+struct AdamWLane {
+    float P[4], G[4], M[4], V[4], R[4];
+    uint32_t mw, rw, mb, rb;  // 8-bit states: codes and scale bytes
+    int64_t i;
+    int live;  // elements that exist
+
+    __device__ __forceinline__ void load(const AdamWSeg &s, int64_t at) {
+        i = at;
+        live = (int)(s.n - i < AW_VEC ? (s.n - i > 0 ? s.n - i : 0) : AW_VEC);
+        const T *p = (const T *)s.p + i, *g = (const T *)s.g + i;
+        const uint8_t *mc = (const uint8_t *)s.m + i, *rc = (const uint8_t *)s.v + i;
+        const float *m = (const float *)s.m + i, *v = (const float *)s.v + i;
+#pragma unroll
+        for (int j = 0; j < 4; j++) P[j] = G[j] = M[j] = V[j] = 0.f;
+        mw = rw = mb = rb = 0;
+        if (live == AW_VEC) {
+            Elems<T>::load4(p, P);
+            Elems<T>::load4(g, G);
+            if (BITS8) {
+                mw = __builtin_nontemporal_load(reinterpret_cast<const u32_u *>(mc));
+                rw = __builtin_nontemporal_load(reinterpret_cast<const u32_u *>(rc));
+            } else {
+                Elems<float>::load4(m, M);
+                Elems<float>::load4(v, V);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (j >= live) continue;
+                P[j] = Elems<T>::load(p + j), G[j] = Elems<T>::load(g + j);
+                if (BITS8) mw |= (uint32_t)mc[j] << 8 * j, rw |= (uint32_t)rc[j] << 8 * j;
+                else M[j] = m[j], V[j] = v[j];
+            }
+        }
+        if (BITS8 && live) mb = s.ms[i / SCALE_BLOCK], rb = s.vs[i / SCALE_BLOCK];
+    }
+
+    __device__ __forceinline__ void step(const AdamWArgs &a, const AdamWSeg &s, float c) {
+        if (BITS8) {
+            const float msc = block_scale(mb), rsc = block_scale(rb);
+            e4m3_decode4(mw, M);
+            e4m3_decode4(rw, R);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                M[j] *= msc;
+                R[j] *= rsc;
+                V[j] = R[j] * R[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) adamw_one(a, s, c, P[j], G[j], M[j], V[j], R[j]);
+        if (BITS8) {
+            uint32_t ma = 0, ra = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {  // of elements that do not exist: zeros, or NaN under a NaN scale
+                ma = max(ma, coded_bits(M[j]));
+                ra = max(ra, coded_bits(R[j]));
+            }
+            mb = scale_byte(row_max(ma));
+            rb = scale_byte(row_max(ra));
+            mw = rw = 0;
+        }
+        if (BITS8 || sizeof(T) == 2) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t w = dither_word((uint64_t)(i + j), s.key);
+                if (BITS8) {
+                    mw |= e4m3_stochastic<true>(M[j], mb, w >> 16) << 8 * j;
+                    rw |= e4m3_stochastic<false>(R[j], rb, w & 0xFFFFu) << 8 * j;
+                }
+                P[j] = Elems<T>::round(P[j], w);
+            }
+        }
+    }
+
+    __device__ __forceinline__ void store(const AdamWSeg &s) const {
+        T *p = (T *)s.p + i;
+        uint8_t *mc = (uint8_t *)s.m + i, *rc = (uint8_t *)s.v + i;
+        float *m = (float *)s.m + i, *v = (float *)s.v + i;
+        if (live == AW_VEC) {
+            Elems<T>::store4(p, P);
+            if (BITS8) {
+                __builtin_nontemporal_store(mw, reinterpret_cast<u32_u *>(mc));
+                __builtin_nontemporal_store(rw, reinterpret_cast<u32_u *>(rc));
+            } else {
+                Elems<float>::store4(m, M);
+                Elems<float>::store4(v, V);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (j >= live) continue;
+                Elems<T>::store(p + j, P[j]);
+                if (BITS8) mc[j] = (uint8_t)(mw >> 8 * j), rc[j] = (uint8_t)(rw >> 8 * j);
+                else m[j] = M[j], v[j] = V[j];
+            }
+        }
+        if (BITS8 && live && i % SCALE_BLOCK == 0) s.ms[i / SCALE_BLOCK] = (uint8_t)mb, s.vs[i / SCALE_BLOCK] = (uint8_t)rb;
+    }
+};
+
 template <typename T, bool BITS8>
 __global__ void __launch_bounds__(AW_THREADS) adamw_kernel(AdamWArgs a) {
     const int k = segment_of(a.block0, a.nseg, (int)blockIdx.x);
     const AdamWSeg &s = a.seg[k];
-    const int64_t n = s.n, i = (int64_t)((int)blockIdx.x - a.block0[k]) * AW_TILE + threadIdx.x * AW_VEC;
+    const int64_t i = (int64_t)((int)blockIdx.x - a.block0[k]) * AW_TILE + threadIdx.x * AW_VEC;
     const float c = a.scale ? *a.scale : 1.f;
-    const int live = (int)(n - i < AW_VEC ? (n - i > 0 ? n - i : 0) : AW_VEC);
-    T *p = (T *)s.p + i;
-    const T *g = (const T *)s.g + i;
-    float P[4] = {0, 0, 0, 0}, G[4] = {0, 0, 0, 0}, M[4] = {0, 0, 0, 0}, V[4] = {0, 0, 0, 0}, R[4];
-    if (live == AW_VEC) {
-        Elems<T>::load4(p, P);
-        Elems<T>::load4(g, G);
-    } else {
-        for (int j = 0; j < live; j++) P[j] = Elems<T>::load(p + j), G[j] = Elems<T>::load(g + j);
-    }
-    if (BITS8) {
-        uint8_t *mc = (uint8_t *)s.m + i, *rc = (uint8_t *)s.v + i;
-        uint32_t mw = 0, rw = 0, mb = 0, rb = 0;
-        if (live) mb = s.ms[i / SCALE_BLOCK], rb = s.vs[i / SCALE_BLOCK];
-        if (live == AW_VEC) {
-            mw = *reinterpret_cast<const u32_u *>(mc), rw = *reinterpret_cast<const u32_u *>(rc);
-        } else {
-            for (int j = 0; j < live; j++) mw |= (uint32_t)mc[j] << 8 * j, rw |= (uint32_t)rc[j] << 8 * j;
-        }
-        e4m3_decode4(mw, M);
-        e4m3_decode4(rw, R);
-        const float msc = block_scale(mb), rsc = block_scale(rb);
-        uint32_t ma = 0, ra = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            M[j] *= msc;
-            R[j] *= rsc;
-            V[j] = R[j] * R[j];
-            adamw_one(a, s, c, P[j], G[j], M[j], V[j], R[j]);
-            ma = max(ma, j < live ? coded_bits(M[j]) : 0u);
-            ra = max(ra, j < live ? coded_bits(R[j]) : 0u);
-        }
-        mb = scale_byte(row_max(ma));
-        rb = scale_byte(row_max(ra));
-        mw = rw = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t w = dither_word((uint64_t)(i + j), s.key);
-            mw |= e4m3_stochastic<true>(M[j], mb, w >> 16) << 8 * j;
-            rw |= e4m3_stochastic<false>(R[j], rb, w & 0xFFFFu) << 8 * j;
-            P[j] = Elems<T>::round(P[j], w);
-        }
-        if (live == AW_VEC) {
-            *reinterpret_cast<u32_u *>(mc) = mw;
-            *reinterpret_cast<u32_u *>(rc) = rw;
-        } else {
-            for (int j = 0; j < live; j++) mc[j] = (uint8_t)(mw >> 8 * j), rc[j] = (uint8_t)(rw >> 8 * j);
-        }
-        if (live && (threadIdx.x & 15) == 0) s.ms[i / SCALE_BLOCK] = (uint8_t)mb, s.vs[i / SCALE_BLOCK] = (uint8_t)rb;
-    } else {
-        float *m = (float *)s.m + i, *v = (float *)s.v + i;
-        if (live == AW_VEC) {
-            Elems<float>::load4(m, M);
-            Elems<float>::load4(v, V);
-        } else {
-            for (int j = 0; j < live; j++) M[j] = m[j], V[j] = v[j];
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            adamw_one(a, s, c, P[j], G[j], M[j], V[j], R[j]);
-            if (sizeof(T) == 2) P[j] = Elems<T>::round(P[j], dither_word((uint64_t)(i + j), s.key));
-        }
-        if (live == AW_VEC) {
-            Elems<float>::store4(m, M);
-            Elems<float>::store4(v, V);
-        } else {
-            for (int j = 0; j < live; j++) m[j] = M[j], v[j] = V[j];
-        }
-    }
-    if (live == AW_VEC) {
-        Elems<T>::store4(p, P);
-    } else {
-        for (int j = 0; j < live; j++) Elems<T>::store(p + j, P[j]);
-    }
+    AdamWLane<T, BITS8> e;
+    e.load(s, i);
+    e.step(a, s, c);
+    e.store(s);
 }
 
 hipError_t launch_adamw(const gsr_adamw_segment *segs, int nseg, int dtype, int state_bits, double beta1, double beta2,
@@ -234,8 +270,8 @@ hipError_t launch_adamw(const gsr_adamw_segment *segs, int nseg, int dtype, int 
 // and sums in 64 bits (the fp64 rate is far above what the stream of gradients needs):
 // no overflow, and the same value whatever the split.  Each workgroup leaves one partial
 // sum; one workgroup adds them in a fixed order.
-constexpr int GN_THREADS = 256, GN_SEGS = 128, GN_BLOCKS = 2048;
-constexpr int GN_TILE = GN_THREADS * 4 * 4;
+constexpr int GN_THREADS = 256, GN_SEGS = 128, GN_BLOCKS = 1024, GN_UNROLL = 4;
+constexpr int64_t gn_tile(int dtype) { return GN_THREADS * GN_UNROLL * (dtype == GSR_DTYPE_F32 ? 4 : 8); }  // 16 KB
 struct NormArgs {
     int nseg, tiles;
     double *partials;
@@ -243,22 +279,33 @@ struct NormArgs {
     gsr_grad_segment seg[GN_SEGS];
 };
 
+__device__ __forceinline__ double add_square(double acc, float x) {
+    return __builtin_fma((double)x, (double)x, acc);
+}
+// 16 bytes of gradients (cached: the step reads them again)
+__device__ __forceinline__ double add_squares(double acc, u32x4_u v, float) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc = add_square(acc, as_f32(v[j]));
+    return acc;
+}
+__device__ __forceinline__ double add_squares(double acc, u32x4_u v, uint16_t) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc = add_square(add_square(acc, as_f32(v[j] << 16)), as_f32(v[j] & 0xFFFF0000u));
+    return acc;
+}
 template <typename T>
 __device__ __forceinline__ double square_sum(const T *g, int64_t n) {
+    constexpr int VEC = 16 / sizeof(T), TILE = GN_THREADS * GN_UNROLL * VEC;
     double acc = 0;
-    if (n >= GN_TILE) {
-        float x[4][4];
+    if (n >= TILE) {
+        u32x4_u v[GN_UNROLL];
 #pragma unroll
-        for (int u = 0; u < 4; u++) Elems<T>::load4(g + (u * GN_THREADS + threadIdx.x) * 4, x[u]);
+        for (int u = 0; u < GN_UNROLL; u++)
+            v[u] = *reinterpret_cast<const u32x4_u *>(g + (u * GN_THREADS + threadIdx.x) * VEC);
 #pragma unroll
-        for (int u = 0; u < 4; u++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) acc = __builtin_fma((double)x[u][j], (double)x[u][j], acc);
+        for (int u = 0; u < GN_UNROLL; u++) acc = add_squares(acc, v[u], T(0));
     } else {
-        for (int64_t i = threadIdx.x; i < n; i += GN_THREADS) {
-            const double x = (double)Elems<T>::load(g + i);
-            acc = __builtin_fma(x, x, acc);
-        }
+        for (int64_t i = threadIdx.x; i < n; i += GN_THREADS) acc = add_square(acc, Elems<T>::load(g + i));
     }
     return acc;
 }
@@ -279,7 +326,7 @@ __global__ void __launch_bounds__(GN_THREADS) grad_norm_kernel(NormArgs a) {
     for (int t = blockIdx.x; t < a.tiles; t += gridDim.x) {
         const int k = segment_of(a.tile0, a.nseg, t);
         const gsr_grad_segment &s = a.seg[k];
-        const int64_t i = (int64_t)(t - a.tile0[k]) * GN_TILE;
+        const int64_t i = (t - a.tile0[k]) * gn_tile(s.dtype);
         acc += s.dtype == GSR_DTYPE_F32 ? square_sum((const float *)s.grad + i, s.n - i)
                                         : square_sum((const uint16_t *)s.grad + i, s.n - i);
     }
@@ -314,7 +361,7 @@ hipError_t launch_grad_norm(const gsr_grad_segment *segs, int nseg, double max_n
         // a launch takes GN_SEGS entries of the list, empty ones too: the scratch holds one
         // set of partial sums for each
         for (int q = 0; q < GN_SEGS && k < nseg; q++, k++) {
-            const int64_t t = (segs[k].n + GN_TILE - 1) / GN_TILE;
+            const int64_t t = (segs[k].n + gn_tile(segs[k].dtype) - 1) / gn_tile(segs[k].dtype);
             if (t == 0) continue;
             a.seg[a.nseg] = segs[k];
             a.tile0[a.nseg++] = a.tiles;

@@ -92,6 +92,7 @@ __device__ __forceinline__ uint32_t dither_word(uint64_t i, uint32_t key) {
 // vectors at their elements' alignment only (views of flat buffers start anywhere):
 // the global loads and stores of gfx950 take them at full width
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint16_t u16x4_u __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32_u __attribute__((aligned(1)));
 typedef uint16_t u16_u __attribute__((aligned(1)));

@@ -436,7 +436,7 @@ __device__ __forceinline__ typename Span<L>::V join(const SpanPlace &p, const ty
 template <int L>
 __device__ __forceinline__ void store_span(uint8_t *dst, int live, const typename Span<L>::V &w) {
     if (live == L) {
-        *reinterpret_cast<typename Span<L>::V_u *>(dst) = w;
+        __builtin_nontemporal_store((typename Span<L>::V_u)w, reinterpret_cast<typename Span<L>::V_u *>(dst));
     } else {
 #pragma unroll
         for (int j = 0; j < L; j++)

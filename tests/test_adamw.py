@@ -151,8 +151,8 @@ def test_grad_norm_abi_refusals(lib):
     assert call((1, 4, 7, 0)) != 0 and "dtype" in _err(lib)
     assert call((None, 4, 0, 0)) != 0 and "NULL" in _err(lib)
     assert lib.gsr_grad_norm(None, 1, 1.0, 1, 1, None) != 0
-    assert lib.gsr_grad_norm_scratch_bytes(1) >= 8 * 2048
-    assert lib.gsr_grad_norm_scratch_bytes(129) >= 2 * 8 * 2048
+    assert lib.gsr_grad_norm_scratch_bytes(1) >= 8 * 1024
+    assert lib.gsr_grad_norm_scratch_bytes(129) >= 2 * 8 * 1024
 
 
 def test_python_refusals_on_cpu():
