@@ -945,7 +945,7 @@ int gsr_select_rows(const float *score, const uint8_t *protect, int32_t P, int32
 int gsr_take_rows(const gsr_rows_segment *segs, int32_t nseg, int64_t P, const int64_t *rows, int64_t K,
                   void *stream) {
     if (nseg < 0 || (nseg > 0 && !segs)) return fail(GSR_ERR_ARGS, "take_rows: bad segment list (%d)", nseg);
-    if (P < 0 || K < 0 || K > INT32_MAX) return fail(GSR_ERR_ARGS, "take_rows: bad P %lld / K %lld", (long long)P, (long long)K);
+    if (P < 0 || P > UINT32_MAX || K < 0 || K > INT32_MAX) return fail(GSR_ERR_ARGS, "take_rows: bad P %lld / K %lld", (long long)P, (long long)K);
     if (K == 0) return GSR_OK;
     if (!rows) return fail(GSR_ERR_ARGS, "take_rows: NULL rows");
     for (int k = 0; k < nseg; k++) {

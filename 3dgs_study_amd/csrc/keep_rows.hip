@@ -96,7 +96,7 @@ __device__ __forceinline__ void pass_state(const SelectArgs &a, uint32_t *sh, ui
 }
 
 // Few workgroups of 16 waves: each ends in one atomic per bin that it met, and with 1024
-// workgroups of four waves those were most of the pass (5M scores: 20 us a pass, now HISTUS).
+// workgroups of four waves those were most of the pass (5M scores: 20 us a pass, now 10).
 // Scores gather in few bins (their exponents), so every bin has SR_COPIES counters, one
 // for every eighth lane, which keeps a wave's additions apart.
 template <int D>
@@ -162,26 +162,34 @@ __global__ void __launch_bounds__(SR_THREADS) select_write_kernel(SelectArgs a) 
         gt0 = block_sum<SR_THREADS>(gt0, sh);
         eq0 = block_sum<SR_THREADS>(eq0, sh);
     }
+    // keys above T in the low half, equal to T in the high half (4096 each at most); the kept
+    // places are lined up in LDS and leave in one run (stored one by one from the lanes that
+    // keep them: 15 us for 5M scores, now 13)
+    __shared__ uint16_t kept[SR_TILE];
+    const int64_t tile0 = (int64_t)blockIdx.x * SR_TILE;
+    uint32_t gt = 0, eq = eq0;
+#pragma unroll
     for (int u = 0; u < SR_TILE / (SR_THREADS * 4); u++) {
-        const int64_t i = (int64_t)blockIdx.x * SR_TILE + (u * SR_THREADS + threadIdx.x) * 4;
+        const uint32_t o = (u * SR_THREADS + threadIdx.x) * 4;
         uint32_t key[4], own = 0, tot;
-        const int live = score_keys(a, i, key);
+        const int live = score_keys(a, tile0 + o, key);
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            if (j < live) own += key[j] > T ? 1u : (key[j] == T ? 0x10000u : 0u);  // gt low, eq high half: <= 1024 each
+            if (j < live) own += key[j] > T ? 1u : (key[j] == T ? 0x10000u : 0u);
         const uint32_t before = block_inclusive_scan<SR_THREADS>(own, sh, &tot) - own;
-        uint32_t g = gt0 + (before & 0xFFFFu), e = eq0 + (before >> 16);
+        uint32_t g = gt + (before & 0xFFFFu), e = eq + (before >> 16);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             if (j >= live) continue;
-            if (key[j] > T) a.rows[g++ + min(e, need)] = i + j;
-            else if (key[j] == T) {
-                if (e < need) a.rows[g + e] = i + j;
-                e++;
-            }
+            if (key[j] > T || (key[j] == T && e < need)) kept[g + min(e, need) - min(eq0, need)] = (uint16_t)(o + j);
+            g += key[j] > T, e += key[j] == T;
         }
-        gt0 += tot & 0xFFFFu, eq0 += tot >> 16;
+        gt += tot & 0xFFFFu, eq += tot >> 16;
     }
+    __syncthreads();
+    const uint32_t n = gt + min(eq, need) - min(eq0, need);
+    int64_t *rows = a.rows + gt0 + min(eq0, need);
+    for (uint32_t i = threadIdx.x; i < n; i += SR_THREADS) rows[i] = tile0 + kept[i];
 }
 
 // Up to SR_SMALL scores: one workgroup, the keys in registers (SR_PER consecutive ones a
@@ -313,17 +321,6 @@ struct TakeArgs {
     int block0[TR_SEGS + 1];
     TakeSeg seg[TR_SEGS];
 };
-
-__device__ __forceinline__ const TakeSeg &take_segment(const TakeArgs &a, int64_t *tile) {
-    int k = 0, hi = a.nseg;
-    while (hi - k > 1) {
-        const int mid = (k + hi) >> 1;
-        if (a.block0[mid] <= (int)blockIdx.x) k = mid;
-        else hi = mid;
-    }
-    *tile = (int)blockIdx.x - a.block0[k];
-    return a.seg[k];
-}
 
 template <typename U>
 __device__ __forceinline__ void take_units(const TakeArgs &a, const TakeSeg &s, int64_t tile) {
@@ -466,19 +463,6 @@ __device__ __forceinline__ void take_spans(const TakeArgs &a, const TakeSeg &s, 
         store_span<16>((uint8_t *)s.dst + u0 + (t * TR_THREADS + threadIdx.x) * 16, p[t].live, join<16>(p[t], A[t], B[t]));
 }
 
-constexpr int TAKE_SPANS = 5;  // else log2 of the unit's bytes
-__global__ void __launch_bounds__(TR_THREADS) take_rows_kernel(TakeArgs a) {
-    int64_t tile;
-    const TakeSeg &s = take_segment(a, &tile);
-    switch (s.kind) {
-        case 0: take_units<uint8_t>(a, s, tile); break;
-        case 1: take_units<uint16_t>(a, s, tile); break;
-        case 2: take_units<uint32_t>(a, s, tile); break;
-        case 3: take_units<uint64_t>(a, s, tile); break;
-        default: take_spans(a, s, tile); break;
-    }
-}
-
 // L codes (in words, the lowest byte first) in units of the scale bytes `sc`, as codes of
 // their new block, which 64 / L lanes of a DPP row hold (every lane of the wave calls): the
 // new scale byte from the largest value, and the values in its units to nearest even by the
@@ -595,18 +579,37 @@ __device__ __forceinline__ void take_codes(const TakeArgs &a, const TakeSeg &s, 
     }
 }
 
-constexpr int TAKE_SIGNED = 1, TAKE_BY_4 = 2, TAKE_BY_16 = 4;
-__global__ void __launch_bounds__(TR_THREADS) take_codes_kernel(TakeArgs a) {
-    int64_t tile;
-    const TakeSeg &s = take_segment(a, &tile);
+// a segment's kind: log2 of the unit's bytes, TAKE_SPANS, or TAKE_CODES and its flags
+constexpr int TAKE_SPANS = 4, TAKE_CODES = 8, TAKE_SIGNED = 1, TAKE_BY_4 = 2, TAKE_BY_16 = 4;
+__global__ void __launch_bounds__(TR_THREADS) take_rows_kernel(TakeArgs a) {
+    int k = 0, hi = a.nseg;
+    while (hi - k > 1) {
+        const int mid = (k + hi) >> 1;
+        if (a.block0[mid] <= (int)blockIdx.x) k = mid;
+        else hi = mid;
+    }
+    const TakeSeg &s = a.seg[k];
+    const int64_t tile = (int)blockIdx.x - a.block0[k];
     switch (s.kind) {
-        case 0: take_codes<false>(a, s, tile); break;
-        case TAKE_SIGNED: take_codes<true>(a, s, tile); break;
-        case TAKE_BY_4: take_code_spans<4, false>(a, s, tile); break;
-        case TAKE_BY_4 + TAKE_SIGNED: take_code_spans<4, true>(a, s, tile); break;
-        case TAKE_BY_16: take_code_spans<16, false>(a, s, tile); break;
+        case 0: take_units<uint8_t>(a, s, tile); break;
+        case 1: take_units<uint16_t>(a, s, tile); break;
+        case 2: take_units<uint32_t>(a, s, tile); break;
+        case 3: take_units<uint64_t>(a, s, tile); break;
+        case TAKE_SPANS: take_spans(a, s, tile); break;
+        case TAKE_CODES: take_codes<false>(a, s, tile); break;
+        case TAKE_CODES + TAKE_SIGNED: take_codes<true>(a, s, tile); break;
+        case TAKE_CODES + TAKE_BY_4: take_code_spans<4, false>(a, s, tile); break;
+        case TAKE_CODES + TAKE_BY_4 + TAKE_SIGNED: take_code_spans<4, true>(a, s, tile); break;
+        case TAKE_CODES + TAKE_BY_16: take_code_spans<16, false>(a, s, tile); break;
         default: take_code_spans<16, true>(a, s, tile); break;
     }
+}
+
+// x / d = x * mul >> (31 + shift) for x < 2^31
+static void divide_by(uint32_t d, uint32_t *mul, uint32_t *shift) {
+    *shift = 0;
+    while ((1ull << *shift) < d) ++*shift;
+    *mul = (uint32_t)(((1ull << (31 + *shift)) + d - 1) / d);
 }
 
 // whether a span of L bytes never touches three rows
@@ -616,55 +619,52 @@ static bool spans_fit(int64_t row, int L) {
     return row + g >= L;
 }
 
+// the segment's table entry; returns its workgroups
+static int64_t take_entry(const gsr_rows_segment &q, int64_t P, int64_t K, TakeSeg *s) {
+    s->src = q.src, s->dst = q.dst, s->src_scale = q.src_scale, s->dst_scale = q.dst_scale;
+    int unit = 0;  // log2 of the bytes
+    int64_t per = TR_BYTES;
+    if (q.kind != GSR_ROWS_PLAIN) {
+        s->kind = TAKE_CODES + (q.kind == GSR_ROWS_E4M3_SIGNED ? TAKE_SIGNED : 0);
+        const bool two = P * q.row_bytes > SCALE_BLOCK;  // the pairs of scales need two blocks in the source
+        if (two && spans_fit(q.row_bytes, 16)) {
+            s->kind += TAKE_BY_16;
+        } else {
+            if (two && spans_fit(q.row_bytes, 4)) s->kind += TAKE_BY_4;
+            per = TR_BYTES / 4;
+        }
+    } else if (spans_fit(q.row_bytes, 16)) {
+        s->kind = TAKE_SPANS;
+    } else {
+        const uint64_t bits = (uint64_t)q.row_bytes | (uint64_t)(uintptr_t)q.src | (uint64_t)(uintptr_t)q.dst;
+        while (unit < 3 && !(bits >> unit & 1)) unit++;
+        s->kind = unit;
+        per = TR_TILE;
+    }
+    s->row = (uint32_t)(q.row_bytes >> unit);
+    s->inv_row = 1.0 / s->row;
+    divide_by(s->row, &s->mul, &s->shift);
+    s->units = K * (int64_t)s->row;
+    return (s->units + per - 1) / per;
+}
+
 hipError_t launch_take_rows(const gsr_rows_segment *segs, int nseg, int64_t P, const int64_t *rows, int64_t K,
                             hipStream_t st) {
     TakeArgs a;
     a.rows = rows, a.P = P;
-    for (int codes = 0; codes < 2; codes++) {
-        for (int k = 0; k < nseg;) {
-            int blocks = 0;
-            a.nseg = 0;
-            for (; k < nseg && a.nseg < TR_SEGS; k++) {
-                const gsr_rows_segment &q = segs[k];
-                if (q.row_bytes == 0 || K == 0 || (q.kind != GSR_ROWS_PLAIN) != (codes != 0)) continue;
-                TakeSeg &s = a.seg[a.nseg];
-                s.src = q.src, s.dst = q.dst, s.src_scale = q.src_scale, s.dst_scale = q.dst_scale;
-                int unit = 0;  // log2 of the bytes
-                int64_t per = TR_BYTES;
-                if (codes) {
-                    s.kind = q.kind == GSR_ROWS_E4M3_SIGNED ? TAKE_SIGNED : 0;
-                    // the pairs of scales need two blocks in the source
-                    const bool two = P * q.row_bytes > SCALE_BLOCK;
-                    if (two && spans_fit(q.row_bytes, 16)) s.kind += TAKE_BY_16;
-                    else {
-                        if (two && spans_fit(q.row_bytes, 4)) s.kind += TAKE_BY_4;
-                        per = TR_BYTES / 4;
-                    }
-                } else if (spans_fit(q.row_bytes, 16)) {
-                    s.kind = TAKE_SPANS;
-                } else {
-                    const uint64_t bits = (uint64_t)q.row_bytes | (uint64_t)(uintptr_t)q.src | (uint64_t)(uintptr_t)q.dst;
-                    while (unit < 3 && !(bits >> unit & 1)) unit++;
-                    s.kind = unit;
-                    per = TR_TILE;
-                }
-                s.row = (uint32_t)(q.row_bytes >> unit);
-                s.inv_row = 1.0 / s.row;
-                s.shift = 0;
-                while ((1ull << s.shift) < s.row) s.shift++;
-                s.mul = (uint32_t)(((1ull << (31 + s.shift)) + s.row - 1) / s.row);
-                s.units = K * (int64_t)s.row;
-                const int64_t b = (s.units + per - 1) / per;
-                if (blocks && blocks + b > GSR_MAX_BLOCKS) break;  // the next launch takes it
-                a.block0[a.nseg++] = blocks;
-                blocks += (int)b;
-            }
-            if (!a.nseg) continue;
-            a.block0[a.nseg] = blocks;
-            if (codes) hipLaunchKernelGGL(take_codes_kernel, dim3(blocks), dim3(TR_THREADS), 0, st, a);
-            else hipLaunchKernelGGL(take_rows_kernel, dim3(blocks), dim3(TR_THREADS), 0, st, a);
-            if (hipError_t e = hipGetLastError()) return e;
+    for (int k = 0; k < nseg;) {
+        int64_t blocks = 0;
+        for (a.nseg = 0; k < nseg && a.nseg < TR_SEGS; k++) {
+            if (segs[k].row_bytes == 0 || K == 0) continue;
+            const int64_t b = take_entry(segs[k], P, K, &a.seg[a.nseg]);
+            if (blocks && blocks + b > GSR_MAX_BLOCKS) break;  // the next launch takes it
+            a.block0[a.nseg++] = (int)blocks;
+            blocks += b;
         }
+        if (!a.nseg) continue;
+        a.block0[a.nseg] = (int)blocks;
+        hipLaunchKernelGGL(take_rows_kernel, dim3((uint32_t)blocks), dim3(TR_THREADS), 0, st, a);
+        if (hipError_t e = hipGetLastError()) return e;
     }
     return hipSuccess;
 }

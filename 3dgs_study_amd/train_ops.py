@@ -246,7 +246,7 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
     are float32 or bfloat16, gradients of the same dtype, all contiguous and on one device.
     8-bit states and bfloat16 parameters are rounded stochastically, by a pure function of
     ``seed`` (an int of up to 64 bits), the tensor's step, its place in the list and the
-    element: the same call gives the same bits.  Step counts, rates and seed are host values
+    element: the same call gives the same bits.  Tensors must not overlap.  Step counts, rates and seed are host values
     and would be frozen in a captured graph: under capture this raises.
 
     Everything is validated before any state is advanced."""
@@ -269,9 +269,9 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
         if not size:
             continue
         addr = p.data_ptr()
-        if addr in seen:
-            raise RuntimeError("adamw_step: a parameter appears twice")
-        seen.add(addr)
+        if addr in seen or m in seen:
+            raise RuntimeError("adamw_step: a parameter or state appears twice")
+        seen.update((addr, m))
         launches.setdefault((dt, bits), []).extend((addr, g.data_ptr(), m, v, ms, vs, size, lrs[k], wds[k],
                                                     st["step"] + 1, k))
     if grad_scale is not None and (grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1 or
@@ -354,6 +354,34 @@ class FusedAdamW:
 
     zero_grad = FusedAdam.zero_grad
 
+    def state_dict(self) -> dict:
+        """{"state": {place: state}, "param_groups": [...]} in torch.optim's form (the tensors
+        themselves, not copies): place counts the parameters through the groups."""
+        params = [p for g in self.param_groups for p in g["params"]]
+        groups, at = [], 0
+        for g in self.param_groups:
+            groups.append({**g, "params": list(range(at, at + len(g["params"])))})
+            at += len(g["params"])
+        return {"state": {k: dict(self.state[p]) for k, p in enumerate(params) if p in self.state},
+                "param_groups": groups}
+
+    def load_state_dict(self, d: dict):
+        """Takes over ``state_dict``'s states (copied to their parameters' device) and the
+        groups' options.  States of either width are taken as they are."""
+        if [len(g["params"]) for g in d["param_groups"]] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError("FusedAdamW.load_state_dict: other param groups")
+        params = [p for g in self.param_groups for p in g["params"]]
+        state = {}
+        for k, st in d["state"].items():
+            p = params[k]
+            st = {n: (x.to(p.device, copy=True) if isinstance(x, torch.Tensor) else x) for n, x in st.items()}
+            st["step"] = int(st["step"])
+            _state_ptrs(st, p, p.numel(), "FusedAdamW.load_state_dict")
+            state[p] = st
+        self.state = state
+        for g, h in zip(self.param_groups, d["param_groups"]):
+            g.update({n: x for n, x in h.items() if n != "params"})
+
     @torch.no_grad()
     def take_rows(self, rows: torch.Tensor, fresh: torch.Tensor = None) -> list:
         """Replaces every parameter by its rows ``rows`` (``take_rows``) and moves its state along;
@@ -421,30 +449,23 @@ def take_rows(tensors, rows: torch.Tensor, states=None):
     dev, at, K = rows.device, rows.get_device(), rows.numel()
     if K >= 1 << 31:
         raise RuntimeError(f"take_rows: at most 2^31 - 1 rows (got {K})")
-    P = None
-    segs, keep = [], []
+    tensors, states = list(tensors), None if states is None else list(states)
+    for t in tensors + [st["exp_avg"] for st in states or ()]:
+        if t.dim():
+            P = t.shape[0]
+            break
+    else:
+        P = 0
+    segs, keep, out, new_states = [], [], [], []
 
-    def shape_of(t):
-        nonlocal P
-        s = t.shape
-        if t.get_device() != at or not s or s[0] != (s[0] if P is None else P):
-            raise RuntimeError(f"take_rows: tensors must have the same number of rows and be on {dev}, got "
-                               f"{tuple(s)} on {t.device}" + ("" if P is None else f" beside {P} rows"))
-        P = s[0]
-        return s
-
-    def plain(t):
-        s = shape_of(t)
-        if not t.is_contiguous():
-            t = t.contiguous()
-            keep.append(t)  # until the launch
-        new = t.new_empty((K, *s[1:]))
-        segs.extend((t.data_ptr(), new.data_ptr(), 0, 0, t.nbytes // P if P else math.prod(s[1:]) * t.element_size(),
-                     _C.ROWS_PLAIN))
-        return new
+    def refuse(t):
+        raise RuntimeError(f"take_rows: tensors must have the same number of rows and be on {dev}, got "
+                           f"{tuple(t.shape)} on {t.device} beside {P} rows")
 
     def coded(codes, src, scale, src_scale, kind):
-        s = shape_of(codes)
+        s = codes.shape
+        if codes.get_device() != at or not s or s[0] != P:
+            refuse(codes)
         row = codes.numel() // P if P else math.prod(s[1:])
         new = codes.new_empty((K, *s[1:]))
         sc = scale.new_empty(-(-K * row // SCALE_BLOCK))
@@ -454,18 +475,33 @@ def take_rows(tensors, rows: torch.Tensor, states=None):
     with _on(dev):
         if not rows.is_contiguous():
             rows = rows.contiguous()
-        out = [plain(t) for t in tensors]
-        new_states = []
+        plain = tensors
         for st in states or ():
             m = st["exp_avg"]
             bits, mp, vp, msp, vsp = _state_ptrs(st, m, m.numel(), "take_rows")
             got = {"step": st["step"]}
+            new_states.append(got)
             if bits == 32:
-                got["exp_avg"], got["exp_avg_sq"] = plain(m), plain(st["exp_avg_sq"])
+                plain = plain + [m, st["exp_avg_sq"]]
             else:
                 got["exp_avg"], got["exp_avg_scale"] = coded(m, mp, st["exp_avg_scale"], msp, _C.ROWS_E4M3_SIGNED)
                 got["exp_rms"], got["exp_rms_scale"] = coded(st["exp_rms"], vp, st["exp_rms_scale"], vsp, _C.ROWS_E4M3)
-            new_states.append(got)
+        for t in plain:
+            s = t.shape
+            if t.get_device() != at or not s or s[0] != P:
+                refuse(t)
+            if not t.is_contiguous():
+                t = t.contiguous()
+                keep.append(t)  # until the launch
+            new = t.new_empty((K, *s[1:]))
+            out.append(new)
+            segs += (t.data_ptr(), new.data_ptr(), 0, 0, t.nbytes // P if P else math.prod(s[1:]) * t.element_size(),
+                     0)  # ROWS_PLAIN
+        moments = iter(out[len(tensors):])
+        del out[len(tensors):]
+        for got in new_states:
+            if len(got) == 1:
+                got["exp_avg"], got["exp_avg_sq"] = next(moments), next(moments)
         if K and segs:
             count = len(segs) // 6  # gsr_rows_segment's fields, the last two as one
             _C._check(lib.gsr_take_rows(struct.pack(f"{6 * count}q", *segs), count, P, rows.data_ptr(), K,

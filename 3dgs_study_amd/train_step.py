@@ -359,7 +359,8 @@ class TrainState:
         the views) so that ``budget`` stay (train_ops.select_rows: ties, NaN, ``protect``): the
         model's six parameters, their optimiser states and the densification statistics are
         replaced by the kept rows, in order.  Returns those rows (int64); the caller's own
-        per-Gaussian tensors follow with train_ops.take_rows.  Needs FusedAdamW."""
+        per-Gaussian tensors follow with train_ops.take_rows; what is bound to the old
+        parameters (a gradient reducer, a captured unit) is made anew.  Needs FusedAdamW."""
         import train_ops
 
         if not isinstance(self.optimizer, train_ops.FusedAdamW):
@@ -401,6 +402,8 @@ def accumulate_blend_weight(camera, gaussians, bg: torch.Tensor, score: torch.Te
     if score.shape != (gaussians.xyz.shape[0],) or score.dtype is not torch.float32:
         raise RuntimeError(f"accumulate_blend_weight: score must be [{gaussians.xyz.shape[0]}] float32, got "
                            f"{tuple(score.shape)} {score.dtype}")
+    if not score.numel():
+        return score
     with torch.enable_grad():
         colours = torch.ones_like(gaussians.xyz).requires_grad_(True)
         image = render(camera, gaussians, bg, override_color=colours)["render"]

@@ -558,7 +558,8 @@ int gsr_select_rows(const float *score, const uint8_t *protect, int32_t P, int32
  * rows[j] is outside [0, P).  Plain segments: rows of row_bytes bytes.  E4M3 segments
  * (gsr_adamw_step's 8-bit states): row_bytes codes a row, whose values are given codes
  * and scales for the blocks that they land in (to nearest even; the magnitudes of
- * GSR_ROWS_E4M3, sqrt(v), never go from nonzero to zero).  dst must not overlap src. */
+ * GSR_ROWS_E4M3, sqrt(v), never go from nonzero to zero).  P < 2^32, K < 2^31, row_bytes
+ * < 2^30, K row_bytes <= 2^34 (2^33 codes).  dst must not overlap src. */
 #define GSR_ROWS_PLAIN 0
 #define GSR_ROWS_E4M3 1
 #define GSR_ROWS_E4M3_SIGNED 2

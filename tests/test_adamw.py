@@ -509,6 +509,7 @@ def test_step_refusals_leave_everything_as_it_was(dev):
         (dict(states=[st, {**st, "exp_avg_scale": st["exp_avg_scale"][:0]}]), "exp_avg_scale"),
         (dict(grad_scale=torch.ones(2, device=dev)), "grad_scale"), (dict(grad_scale=torch.ones(())), "grad_scale"),
         (dict(betas=(0.9, 1.0)), "betas"), (dict(eps=-1.0), "eps"),
+        (dict(states=[st, st]), "twice"),
     ]
     q = torch.randn(8, 4, device=dev)
     for kw, msg in cases:
@@ -667,3 +668,46 @@ def test_train_state_runs_with_8_bit_states(dev):
         assert float((d > 1e-3 * lr + 4 * U * a.abs()).float().mean()) < 1e-2
         assert float(d.max()) <= 2 * lr + 1e-6
     np.testing.assert_allclose(float(got[32][1]), float(got[8][1]), rtol=1e-4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_dict_round_trip(dev, bits, tmp_path):
+    """Saved, loaded with the safe loader into another optimiser, and continued: the same bits."""
+    import train_ops
+
+    gen = torch.Generator().manual_seed(0)
+    base = [torch.randn(77, 3, generator=gen), torch.randn(5, generator=gen), torch.randn(0, 3)]
+    grads = [[torch.randn(b.shape, generator=gen).to(dev) for b in base] for _ in range(4)]
+
+    def make():
+        ps = [b.clone().to(dev).requires_grad_(True) for b in base]
+        return ps, train_ops.FusedAdamW([{"params": ps[:2], "lr": 0.1, "name": "a"}, {"params": ps[2:]}],
+                                        state_bits=bits, weight_decay=0.1, max_norm=1.0, seed=5)
+
+    def run(ps, opt, steps):
+        for k in steps:
+            for p, g in zip(ps, grads[k]):
+                p.grad = g
+            opt.step()
+
+    pa, oa = make()
+    run(pa, oa, range(2))
+    path = tmp_path / "opt.pt"
+    torch.save(oa.state_dict(), path)
+    pb, ob = make()
+    for p, q in zip(pa, pb):
+        q.data.copy_(p.data)
+    ob.param_groups[0]["lr"] = 0.5
+    ob.load_state_dict(torch.load(path, weights_only=True))
+    assert ob.param_groups[0]["lr"] == 0.1 and ob.param_groups[0]["name"] == "a"
+    run(pa, oa, range(2, 4))
+    run(pb, ob, range(2, 4))
+    for p, q in zip(pa, pb):
+        assert torch.equal(p, q) and oa.state[p]["step"] == ob.state[q]["step"] == 4
+    with pytest.raises(ValueError, match="param groups"):
+        ob.load_state_dict({"state": {}, "param_groups": []})
+    bad = oa.state_dict()
+    bad["state"][0]["exp_avg"] = bad["state"][0]["exp_avg"][:5]
+    with pytest.raises(RuntimeError, match="exp_avg"):
+        ob.load_state_dict(bad)

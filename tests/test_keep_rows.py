@@ -84,6 +84,7 @@ def test_take_rows_abi_refusals(lib):
     ok = (1, 1, None, None, 12, 0, 0)
     assert f(ok, n=-1) != 0 and "segment list" in _err(lib)
     assert f(ok, P=-1) != 0 and "bad P" in _err(lib)
+    assert f(ok, P=1 << 32) != 0 and "bad P" in _err(lib)
     assert f(ok, K=-1) != 0 and f(ok, K=1 << 31) != 0 and "K" in _err(lib)
     assert f(ok, rows=None) != 0 and "NULL" in _err(lib)
     assert f((None,) + ok[1:]) != 0 and "NULL" in _err(lib)
@@ -153,7 +154,7 @@ def test_select_rows_exact(dev, P, kind):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("P", [300_000, 5_000_011])
+@pytest.mark.parametrize("P", [16_384, 16_385, 300_000, 5_000_011, 17_000_003])
 def test_select_rows_large(dev, P):
     import train_ops
 
