@@ -7,6 +7,7 @@
 // here: every buffer belongs to the caller (torch's caching allocator on the
 // Python side).  The only host synchronisation is the num_rendered read-back
 // in gsr_forward_preprocess, as upstream.
+#include <cfloat>
 #include <atomic>
 #include <chrono>
 #include <cstdarg>
@@ -903,6 +904,7 @@ int gsr_adamw_step(const gsr_adamw_segment *segs, int32_t nseg, int32_t dtype, i
     if (state_bits != 32 && state_bits != 8) return fail(GSR_ERR_ARGS, "adamw: state_bits must be 32 or 8 (got %d)", state_bits);
     if (!(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0))
         return fail(GSR_ERR_ARGS, "adamw: betas must be in [0, 1) and eps >= 0");
+    if (eps > 0 && (float)eps < FLT_MIN) return fail(GSR_ERR_ARGS, "adamw: eps must be 0 or a normal float (got %g)", eps);
     for (int k = 0; k < nseg; k++) {
         const gsr_adamw_segment &q = segs[k];
         if (q.n < 0 || q.n > (int64_t)1 << 33) return fail(GSR_ERR_ARGS, "adamw: bad size %lld in segment %d", (long long)q.n, k);

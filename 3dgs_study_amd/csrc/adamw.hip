@@ -107,7 +107,8 @@ __device__ __forceinline__ void adamw_one(const AdamWArgs &a, const AdamWSeg &s,
     m = m + (x - m) * a.w1;
     v = v * a.b2 + (x * x) * a.w2;
     r = sqrtf(v);
-    p = p * s.decay + (m / (r * s.inv_bc2 + a.eps)) * s.neg_step;
+    // the quotient by the hardware's reciprocal (1 ulp): nothing is rounded to few bits from it
+    p = p * s.decay + (m * __builtin_amdgcn_rcpf(r * s.inv_bc2 + a.eps)) * s.neg_step;
 }
 
 // Four consecutive elements of a segment, as a lane holds them
@@ -166,24 +167,43 @@ struct AdamWLane {
         if (BITS8) {
             uint32_t ma = 0, ra = 0;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {  // of elements that do not exist: zeros, or NaN under a NaN scale
+            for (int j = 0; j < 4; j++) {
+                ma = max(ma, as_u32(M[j]) & 0x7FFFFFFFu);
+                ra = max(ra, as_u32(R[j]) & 0x7FFFFFFFu);
+            }
+            // a moment past the codes' range anywhere in the wave: every element is tested
+            if (__any(max(ma, ra) >= E4M3_TOP)) {
+                encode<true>(s);
+            } else {
+                mb = scale_byte(row_max(ma));
+                rb = scale_byte(row_max(ra));
+                encode<false>(s);
+            }
+        } else if (sizeof(T) == 2) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) P[j] = Elems<T>::round(P[j], dither_word((uint64_t)(i + j), s.key));
+        }
+    }
+
+    template <bool TEST>
+    __device__ __forceinline__ void encode(const AdamWSeg &s) {
+        if (TEST) {
+            uint32_t ma = 0, ra = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
                 ma = max(ma, coded_bits(M[j]));
                 ra = max(ra, coded_bits(R[j]));
             }
             mb = scale_byte(row_max(ma));
             rb = scale_byte(row_max(ra));
-            mw = rw = 0;
         }
-        if (BITS8 || sizeof(T) == 2) {
+        mw = rw = 0;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint32_t w = dither_word((uint64_t)(i + j), s.key);
-                if (BITS8) {
-                    mw |= e4m3_stochastic<true>(M[j], mb, w >> 16) << 8 * j;
-                    rw |= e4m3_stochastic<false>(R[j], rb, w & 0xFFFFu) << 8 * j;
-                }
-                P[j] = Elems<T>::round(P[j], w);
-            }
+        for (int j = 0; j < 4; j++) {
+            const uint32_t w = dither_word((uint64_t)(i + j), s.key);
+            mw |= e4m3_stochastic<true, TEST>(M[j], mb, w >> 16) << 8 * j;
+            rw |= e4m3_stochastic<false, TEST>(R[j], rb, w & 0xFFFFu) << 8 * j;
+            P[j] = Elems<T>::round(P[j], w);
         }
     }
 

@@ -54,24 +54,20 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v) {
 }
 __device__ __forceinline__ uint32_t scale_byte(uint32_t amax) { return (uint32_t)max((int)(amax >> 23) - 7, 0); }
 
-// the code of x under the scale byte.  SIGNED: the first moment; else magnitudes (the
-// root of the second moment), of which none but zero may become zero: it divides
-template <bool SIGNED>
-__device__ __forceinline__ uint32_t e4m3_round(float x, uint32_t u, uint32_t round) {
+// The code of x under the scale byte, rounded up where 16 random bits, centred in the 20 that
+// are dropped, carry.  SIGNED: the first moment; else magnitudes (the root of the second
+// moment), of which none but zero may become zero: it divides.  TEST: x may be past the
+// codes' range.
+template <bool SIGNED, bool TEST>
+__device__ __forceinline__ uint32_t e4m3_stochastic(float x, uint32_t byte, uint32_t dither) {
     const uint32_t bits = as_u32(x), a = bits & 0x7FFFFFFFu;
-    uint32_t c = (u + round) >> 20;
-    if (!SIGNED) c = a ? max(c, 1u) : 0u;
-    c = a < E4M3_TOP ? c : 0x7Fu;
+    const float v = TEST ? as_f32(coded_bits(x)) : __builtin_fabsf(x);
+    uint32_t c = (as_u32(__builtin_ldexpf(v, 7 - (int)byte)) + (dither << 4 | 8u)) >> 20;
+    if (!SIGNED) c = max(c, min(a, 1u));
+    if (TEST) c = a < E4M3_TOP ? c : 0x7Fu;
     return SIGNED ? c | ((bits >> 24) & 0x80u) : c;
 }
-__device__ __forceinline__ uint32_t e4m3_units(float x, uint32_t byte) {
-    return as_u32(__builtin_ldexpf(as_f32(coded_bits(x)), 7 - (int)byte));
-}
-// dither: 16 random bits, centred in the 20 that are dropped
-template <bool SIGNED>
-__device__ __forceinline__ uint32_t e4m3_stochastic(float x, uint32_t byte, uint32_t dither) {
-    return e4m3_round<SIGNED>(x, e4m3_units(x, byte), dither << 4 | 8u);
-}
+
 // A 32-bit mixing (xor-shifts and odd multipliers: the fractional bits of the roots of
 // 2 and 3), and the random word of element i of a tensor from the tensor's key: a pure
 // function, so a run repeats and every replica of a data-parallel job rounds alike.

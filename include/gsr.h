@@ -514,7 +514,7 @@ int gsr_adam_step(const gsr_adam_segment *segs, int32_t nseg, int32_t step, doub
  * with ceil(n / 64) scale bytes; a state of all zero bytes is the initial one.  Codes
  * and bf16 parameters are rounded stochastically, from a pure function of (seed, step,
  * ordinal, element).  A moment that is NaN or 2^127 or more becomes its element's NaN code.
- * n <= 2^33 per segment.  Segments must not overlap. */
+ * n <= 2^33 per segment; eps is 0 or a normal float.  Segments must not overlap. */
 #define GSR_DTYPE_F32 0
 #define GSR_DTYPE_BF16 1
 typedef struct {

@@ -9,8 +9,8 @@ Tolerances, with u = 2^-24 (half a step of fp32, relative):
   r' = sqrt(v'): half of that and its own u: 4 u r'.
   d  = r' inv + eps: r's 4 u, u each for inv, the product, eps and the sum: 8 u d.
   p' = p decay + (m'/d) step: 3 u |p| for the first term and its place in the sum; the update
-       carries |m' error| step / d, and 8 u (d) + u (quotient) + u (step) + u (product) +
-       u (sum) = 12 u of itself.
+       carries |m' error| step / d, and 8 u (d) + 2 u (the reciprocal's 1 ulp) + u (product
+       with m') + u (step) + u (product) + u (sum) = 14 u of itself.
 e4m3 codes are rounded to one of the two neighbours: less than one step, 2^-3 of the value's
 power of two, 2^-9 of the scale below 2^-6 of it."""
 import ctypes
@@ -69,7 +69,7 @@ def _exact(p, g, m, v, lr, wd, t, c=1.0, betas=(0.9, 0.999), eps=1e-15):
     k = lr / (1 - b1 ** t)
     up = k * m2 / d
     em = 5 * U * (m.abs() + x.abs())
-    return (p * (1 - lr * wd) - up, m2, v2), (3 * U * p.abs() + k * em / d + 12 * U * up.abs(), em, 6 * U * v2)
+    return (p * (1 - lr * wd) - up, m2, v2), (3 * U * p.abs() + k * em / d + 14 * U * up.abs(), em, 6 * U * v2)
 
 
 def _within(got, want, bound, what):
@@ -128,6 +128,7 @@ def test_adamw_abi_refusals(lib):
     assert call([ok], b1=1.0) != 0 and "betas" in _err(lib)
     assert call([ok], b2=math.nan) != 0 and "betas" in _err(lib)
     assert call([ok], eps=-1.0) != 0
+    assert call([ok], eps=1e-40) != 0 and "eps" in _err(lib)  # the reciprocal takes normal numbers
     assert call([ok[:9] + (0, 0)]) != 0 and "step" in _err(lib)
     assert call([ok[:6] + (-1,) + ok[7:]]) != 0 and "size" in _err(lib)
     assert call([ok[:6] + ((1 << 33) + 1,) + ok[7:]]) != 0 and "size" in _err(lib)
