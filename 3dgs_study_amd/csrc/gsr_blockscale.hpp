@@ -9,11 +9,10 @@
 // mantissa, and rescaling is exact; one binade below the top, so that rounding up
 // never reaches past 256 and nothing saturates.  2^17 of range is left below it.
 //
-// Encoding: u = |x| 2^(7 - byte) puts e4m3's smallest normal value (2^-6, in units
-// of the scale) on fp32's smallest normal (2^-126): e4m3's subnormals are then fp32's,
-// and code = (bits(u) + round) >> 20 for every magnitude, with
-//   round = 20 random bits (stochastic: the expected value is u), or
-//   round = 0x7FFFF + the code's last bit (to nearest, ties to even).
+// Encoding by hand (the stochastic rounding of the optimiser step): u = |x| 2^(7 - byte)
+// puts e4m3's smallest normal value (2^-6, in units of the scale) on fp32's smallest
+// normal (2^-126).  e4m3's subnormals are then fp32's, and code = (bits(u) + 20 random
+// bits) >> 20 for every magnitude: the expected value is u.
 // A 16-lane DPP row holds one block, 4 elements a lane.
 #pragma once
 

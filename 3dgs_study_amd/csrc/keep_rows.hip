@@ -8,6 +8,8 @@
 // largest key T and how many of the keys equal to T stay; those of the lowest index do.
 // The kept rows are then counted per tile, the counts scanned, and the indices written in
 // order.  All counts are integers: the result does not depend on the order of the atomics.
+// Six launches, 33 us for 1M scores and 53 us for 5M (the scores are read five times, from
+// the caches); up to 16384 scores one workgroup does it all (10k: 14 us, 28 us by the six).
 #include "gsr_blockscale.hpp"
 #include "gsr_kernels.hpp"
 #include "gsr_wave.hpp"
@@ -287,6 +289,10 @@ hipError_t launch_select_rows(const float *score, const uint8_t *protect, int P,
 // long, so that its bytes arrive in their place and a mask joins the two.  Where a load would
 // leave the source (its first and last rows) the lane reads its bytes one by one.  Rows that
 // are too short for it (4-byte rows: opacities) move one unit a lane.
+// Memory bounds it, counted in whole lines, those of dropped rows among them: 1M -> 500k
+// Gaussians with fp32 states 152 us (unit by unit: 198), 5M -> 3M with 8-bit states 600 us
+// (3.1 GB moved, 5.1 TB/s; a byte or a word of codes a lane: 850 us).  Stored non-temporally
+// (164 -> 152 us), loaded through the caches, which hold the neighbouring rows' part of a line.
 //
 // 8-bit states (gsr_blockscale.hpp): the rows' values land in other blocks of 64, whose
 // scale is formed anew from what they hold; powers of two, so only values below 2^-13 of
