@@ -214,7 +214,7 @@ def _state_ptrs(st: dict, p: torch.Tensor, n: int, who: str) -> tuple:
 
 
 def _per_tensor(x, n: int, name: str) -> list:
-    if isinstance(x, (int, float)):
+    if not isinstance(x, (list, tuple)):
         return [float(x)] * n
     if len(x) != n:
         raise ValueError(f"adamw_step: {len(x)} values of {name} for {n} tensors")
@@ -277,9 +277,9 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
     if grad_scale is not None and (grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1 or
                                    grad_scale.device != dev):
         raise RuntimeError(f"adamw_step: grad_scale must be a float32 scalar on {dev}")
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("adamw_step: step counts and rates are host values; not for graph capture")
     with _on(dev):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("adamw_step: step counts and rates are host values; not for graph capture")
         for (dt, bits), segs in launches.items():
             count = len(segs) // 11  # gsr_adamw_segment's fields
             _C._check(lib.gsr_adamw_step(struct.pack("7q2d2i" * count, *segs), count, _C.DTYPES[dt], bits, betas[0],
@@ -287,7 +287,7 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
                                          seed & 0xFFFFFFFFFFFFFFFF, _C._stream(dev)), "gsr_adamw_step")
     for st in states:
         st["step"] += 1
-    torch.autograd.graph.increment_version(params)
+    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
 
 
 def grad_norm(grads, max_norm: float = math.inf):
@@ -393,11 +393,14 @@ class FusedAdamW:
         if fresh is None:
             new, states = take_rows(params, rows, [self.state[p] for p in have])
         else:
+            if fresh.dtype is not torch.bool or fresh.shape != rows.shape:
+                raise RuntimeError(f"FusedAdamW.take_rows: fresh must be {rows.numel()} bools, got {fresh.dtype} "
+                                   f"{tuple(fresh.shape)}")
             new = take_rows(params, rows)
             _, states = take_rows([], torch.where(fresh, -1, rows), [self.state[p] for p in have])
+        new = [torch.nn.Parameter(q, p.requires_grad) if isinstance(p, torch.nn.Parameter) else
+               q.requires_grad_(p.requires_grad) for p, q in zip(params, new)]
         old = dict(zip(params, new))
-        for p, q in old.items():
-            q.requires_grad_(p.requires_grad)
         self.state = {old[p]: st for p, st in zip(have, states)}
         for g in self.param_groups:
             g["params"] = [old[p] for p in g["params"]]
@@ -490,8 +493,8 @@ def take_rows(tensors, rows: torch.Tensor, states=None):
             s = t.shape
             if t.get_device() != at or not s or s[0] != P:
                 refuse(t)
-            if not t.is_contiguous():
-                t = t.contiguous()
+            if not t.is_contiguous() or t.is_conj() or t.is_neg():
+                t = t.resolve_conj().resolve_neg().contiguous()
                 keep.append(t)  # until the launch
             new = t.new_empty((K, *s[1:]))
             out.append(new)

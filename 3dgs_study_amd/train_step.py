@@ -399,13 +399,14 @@ def accumulate_blend_weight(camera, gaussians, bg: torch.Tensor, score: torch.Te
     i's colour enters the pixel: the gradient of the image's first channel with respect to
     the Gaussians' (overridden) colours, from the rasterizer's own backward.  ``score``:
     [P] float32, in place."""
-    if score.shape != (gaussians.xyz.shape[0],) or score.dtype is not torch.float32:
-        raise RuntimeError(f"accumulate_blend_weight: score must be [{gaussians.xyz.shape[0]}] float32, got "
+    xyz = gaussians.get_xyz
+    if score.shape != xyz.shape[:1] or score.dtype is not torch.float32:
+        raise RuntimeError(f"accumulate_blend_weight: score must be [{xyz.shape[0]}] float32, got "
                            f"{tuple(score.shape)} {score.dtype}")
     if not score.numel():
         return score
     with torch.enable_grad():
-        colours = torch.ones_like(gaussians.xyz).requires_grad_(True)
+        colours = torch.ones_like(xyz).requires_grad_(True)
         image = render(camera, gaussians, bg, override_color=colours)["render"]
         seed = torch.zeros_like(image)
         seed[0] = 1.0

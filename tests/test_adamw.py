@@ -540,6 +540,18 @@ def test_step_raises_for_a_graph_that_saved_the_parameter(dev):
 
 
 @pytest.mark.gpu
+def test_step_takes_numpy_rates_and_inference_tensors(dev):
+    import train_ops
+
+    with torch.inference_mode():
+        p = torch.ones(5, device=dev)
+        train_ops.adamw_step([p], [torch.ones(5, device=dev)], [train_ops.adamw_state(p)], np.float32(0.5),
+                             weight_decay=np.float64(0.0))
+        # the first step is lr g / |g|, to 2^-23 of its roundings
+        np.testing.assert_allclose(p.cpu().numpy(), 0.5, rtol=1e-5)
+
+
+@pytest.mark.gpu
 def test_step_on_another_stream(dev):
     import train_ops
 

@@ -310,6 +310,40 @@ def test_rows_refusals_on_gpu(dev):
 
 
 @pytest.mark.gpu
+def test_take_rows_of_conjugate_and_negated_views(dev):
+    """Views whose values differ from their bytes."""
+    import train_ops
+
+    z = torch.complex(torch.arange(12.0), torch.arange(1.0, 13.0)).view(6, 2).to(dev)
+    rows = torch.tensor([4, 0, 4], device=dev)
+    ts = [z.conj(), z.conj().imag, z]
+    for t, got in zip(ts, train_ops.take_rows(ts, rows)):
+        assert torch.equal(torch.view_as_real(got.resolve_conj()) if got.is_complex() else got,
+                           torch.view_as_real(t[rows].resolve_conj()) if t.is_complex() else t[rows].resolve_neg())
+
+
+@pytest.mark.gpu
+def test_optimizer_take_rows_keeps_parameters_what_they_are(dev):
+    import train_ops
+
+    p, q = torch.nn.Parameter(torch.randn(6, 2, device=dev)), torch.randn(6, device=dev)
+    opt = train_ops.FusedAdamW([{"params": [p], "lr": 0.1}, {"params": [q], "lr": 0.1}], state_bits=8)
+    p.grad = torch.ones_like(p)
+    opt.step()  # q has no state
+    rows = torch.tensor([5, 0, 5], device=dev)
+    for bad in (torch.ones(3, device=dev), torch.ones(1, dtype=torch.bool, device=dev)):
+        with pytest.raises(RuntimeError, match="fresh"):
+            opt.take_rows(rows, bad)
+    new = opt.take_rows(rows)
+    assert isinstance(new[0], torch.nn.Parameter) and new[0].requires_grad and not new[1].requires_grad
+    assert torch.equal(new[0], p[rows]) and torch.equal(new[1], q[rows])
+    assert list(opt.state) == [new[0]] and opt.param_groups[1]["params"][0] is new[1]
+    new[0].grad = torch.ones_like(new[0])
+    opt.step()
+    assert opt.state[new[0]]["step"] == 2
+
+
+@pytest.mark.gpu
 def test_select_and_take_captured_and_replayed(dev):
     """Both in one graph (no host wait, the kept count is known), replayed over new scores with
     eager work between, and on a side stream."""
