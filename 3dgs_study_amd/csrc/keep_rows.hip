@@ -8,7 +8,7 @@
 // largest key T and how many of the keys equal to T stay; those of the lowest index do.
 // The kept rows are then counted per tile, the counts scanned, and the indices written in
 // order.  All counts are integers: the result does not depend on the order of the atomics.
-// Six launches, 33 us for 1M scores and 53 us for 5M (the scores are read five times, from
+// Six launches, 37 us for 1M scores and 53 us for 5M (the scores are read five times, from
 // the caches); up to 16384 scores one workgroup does it all (10k: 14 us, 28 us by the six).
 #include "gsr_blockscale.hpp"
 #include "gsr_kernels.hpp"
