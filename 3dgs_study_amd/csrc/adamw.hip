@@ -14,8 +14,8 @@
 // Memory bounds it: 28 bytes an element with 32-bit states, 16 with 8-bit ones.  59M
 // elements (1M Gaussians): 265 us = 6.2 TB/s and 150 us = 6.3 TB/s, where a large copy
 // reaches 4.75 and an addition of two arrays 5.85.  All of it streams non-temporally: 304
-// and 165 us with ordinary accesses, 274 us with the parameters alone kept in the caches
-// (too large to be there at the next render).  Two or four vectors a lane: 314, 316 us.
+// us (32 bits) with ordinary accesses, 274 with the parameters alone kept in the caches (too
+// large to be there at the next render).  Two or four vectors a lane: 314, 316 us.
 //
 // 8-bit states hold m and r = sqrt(v) (half the range of v's exponents) as e4m3 codes
 // with a power-of-two scale for every 64 elements (gsr_blockscale.hpp).  They are

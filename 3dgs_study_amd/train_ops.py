@@ -499,7 +499,7 @@ def take_rows(tensors, rows: torch.Tensor, states=None):
             new = t.new_empty((K, *s[1:]))
             out.append(new)
             segs += (t.data_ptr(), new.data_ptr(), 0, 0, t.nbytes // P if P else math.prod(s[1:]) * t.element_size(),
-                     0)  # ROWS_PLAIN
+                     _C.ROWS_PLAIN)
         moments = iter(out[len(tensors):])
         del out[len(tensors):]
         for got in new_states:
