@@ -246,10 +246,11 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
     are float32 or bfloat16, gradients of the same dtype, all contiguous and on one device.
     8-bit states and bfloat16 parameters are rounded stochastically, by a pure function of
     ``seed`` (an int of up to 64 bits), the tensor's step, its place in the list and the
-    element: the same call gives the same bits.  Tensors must not overlap.  Step counts, rates and seed are host values
-    and would be frozen in a captured graph: under capture this raises.
+    element: the same call gives the same bits.  Tensors must not overlap.  Step counts,
+    rates and seed are host values and would be frozen in a captured graph: under capture
+    this raises.
 
-    Everything is validated before any state is advanced."""
+    Everything is validated before anything is launched and any count advanced."""
     lib = _C.load_library()
     n = len(params)
     if len(grads) != n or len(states) != n:
@@ -280,11 +281,13 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
     with _on(dev):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("adamw_step: step counts and rates are host values; not for graph capture")
-        for (dt, bits), segs in launches.items():
-            count = len(segs) // 11  # gsr_adamw_segment's fields
-            _C._check(lib.gsr_adamw_step(struct.pack("7q2d2i" * count, *segs), count, _C.DTYPES[dt], bits, betas[0],
-                                         betas[1], eps, None if grad_scale is None else grad_scale.data_ptr(),
-                                         seed & 0xFFFFFFFFFFFFFFFF, _C._stream(dev)), "gsr_adamw_step")
+        stream, scale = _C._stream(dev), None if grad_scale is None else grad_scale.data_ptr()
+        seed &= 0xFFFFFFFFFFFFFFFF
+        tables = [(kind, struct.pack("7q2d2i" * (len(segs) // 11), *segs), len(segs) // 11)  # gsr_adamw_segment
+                  for kind, segs in launches.items()]
+        for (dt, bits), table, count in tables:
+            _C._check(lib.gsr_adamw_step(table, count, _C.DTYPES[dt], bits, betas[0], betas[1], eps, scale, seed,
+                                         stream), "gsr_adamw_step")
     for st in states:
         st["step"] += 1
     torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])

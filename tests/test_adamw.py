@@ -540,6 +540,20 @@ def test_step_raises_for_a_graph_that_saved_the_parameter(dev):
 
 
 @pytest.mark.gpu
+def test_step_a_bad_count_in_one_launch_stops_all(dev):
+    import struct
+
+    import train_ops
+
+    ps = [torch.ones(5, device=dev), torch.ones(5, device=dev)]
+    st = [train_ops.adamw_state(ps[0]), train_ops.adamw_state(ps[1], 8)]
+    st[1]["step"] = 2 ** 31 - 1
+    with pytest.raises(struct.error):
+        train_ops.adamw_step(ps, [p.clone() for p in ps], st, 0.1)
+    assert st[0]["step"] == 0 and all(torch.equal(p, torch.ones_like(p)) for p in ps)
+
+
+@pytest.mark.gpu
 def test_step_takes_numpy_rates_and_inference_tensors(dev):
     import train_ops
 

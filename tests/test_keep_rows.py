@@ -344,6 +344,33 @@ def test_optimizer_take_rows_keeps_parameters_what_they_are(dev):
 
 
 @pytest.mark.gpu
+def test_two_streams_at_once(dev):
+    """Norm, selection and gather on two streams side by side: each call has scratch of its own."""
+    import train_ops
+
+    P, K = 200_003, 70_000
+    ins = [(torch.rand(P, device=dev), torch.randn(P, 45, device=dev), _state8((P, 3), k, dev)) for k in range(2)]
+
+    def go(score, x, st):
+        norm, scale = train_ops.grad_norm([x], 1.0)
+        rows = train_ops.select_rows(score, K)
+        (y,), (q,) = train_ops.take_rows([x], rows, [st])
+        return [norm, scale, rows, y] + [q[k].view(torch.uint8) for k in q if k != "step"]
+
+    want = [go(*i) for i in ins]
+    streams = [torch.cuda.Stream() for _ in ins]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(go(*ins[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(a, b) for g in got[k] for a, b in zip(g, want[k]))
+
+
+@pytest.mark.gpu
 def test_select_and_take_captured_and_replayed(dev):
     """Both in one graph (no host wait, the kept count is known), replayed over new scores with
     eager work between, and on a side stream."""
