@@ -146,6 +146,7 @@ _KEYS = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_scale", "exp_rms
 
 
 _SAME = contextlib.nullcontext()
+_F32, _CODE, _SCALE = torch.float32, torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
 def _on(device):
@@ -185,27 +186,29 @@ def _state_refuse(st: dict, p: torch.Tensor, who: str):
     for k in _KEYS[bits]:
         t = st.get(k)
         scale = k.endswith("_scale")
-        want = torch.float32 if bits == 32 else (torch.float8_e8m0fnu if scale else torch.float8_e4m3fn)
+        want = _F32 if bits == 32 else (_SCALE if scale else _CODE)
         if t is None or t.dtype is not want or t.numel() != (-(-n // SCALE_BLOCK) if scale else n) or \
-                t.device != p.device or not t.is_contiguous():
-            raise RuntimeError(f"{who}: state {k!r} must be contiguous {want} on {p.device} and fit its "
-                               f"parameter of {tuple(p.shape)}" + ("" if t is None else
+                t.device != p.device or not t.is_contiguous() or t.is_neg():
+            raise RuntimeError(f"{who}: state {k!r} must be contiguous {want} on {p.device}, no negated view, and fit "
+                               f"its parameter of {tuple(p.shape)}" + ("" if t is None else
                                f" (got {t.dtype} {tuple(t.shape)} on {t.device})"))
 
 
-def _state_ptrs(st: dict, p: torch.Tensor, n: int, who: str) -> tuple:
-    """(bits, then exp_avg, exp_second and their scales' addresses) of a checked state of ``p``."""
+def _state_ptrs(st: dict, p: torch.Tensor, n: int, who: str, raw: bool = True) -> tuple:
+    """(bits, then exp_avg, exp_second and their scales' addresses) of a checked state of ``p``.
+    ``raw``: its bytes are read (codes have no negated views: those come of complex numbers)."""
     at = p.get_device()
     v = st.get("exp_avg_sq")
     m = st.get("exp_avg")
     if v is not None:
-        if m is None or not (m.dtype is v.dtype is torch.float32 and m.numel() == n == v.numel() and
-                             m.get_device() == at == v.get_device() and m.is_contiguous() and v.is_contiguous()):
+        if m is None or not (m.dtype is v.dtype is _F32 and m.numel() == n == v.numel() and
+                             m.get_device() == at == v.get_device() and m.is_contiguous() and v.is_contiguous()) or \
+                raw and (m.is_neg() or v.is_neg()):
             _state_refuse(st, p, who)
         return 32, m.data_ptr(), v.data_ptr(), 0, 0
     r, ms, rs = st.get("exp_rms"), st.get("exp_avg_scale"), st.get("exp_rms_scale")
     if m is None or r is None or ms is None or rs is None or not (
-            m.dtype is r.dtype is torch.float8_e4m3fn and ms.dtype is rs.dtype is torch.float8_e8m0fnu and
+            m.dtype is r.dtype is _CODE and ms.dtype is rs.dtype is _SCALE and
             m.numel() == n == r.numel() and ms.numel() == rs.numel() == -(-n // SCALE_BLOCK) and
             m.get_device() == r.get_device() == ms.get_device() == rs.get_device() == at and
             m.is_contiguous() and r.is_contiguous() and ms.is_contiguous() and rs.is_contiguous()):
@@ -231,6 +234,8 @@ def _adamw_refuse(p: torch.Tensor, g: torch.Tensor, dev):
         raise RuntimeError(f"adamw_step: tensors on {p.device} and {g.device}, expected {dev}")
     if g.shape != p.shape:
         raise RuntimeError(f"adamw_step: gradient {tuple(g.shape)} of a parameter {tuple(p.shape)}")
+    if p.is_neg():
+        raise RuntimeError("adamw_step: parameters must not be negated views")
     raise RuntimeError("adamw_step: parameters and gradients must be contiguous")
 
 
@@ -243,7 +248,8 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
     ``lr`` and ``weight_decay``: a number, or one per tensor.  Each state's ``step`` counts
     its own tensor's steps and is advanced by one.  ``grad_scale``: a float32 scalar on the
     device that every gradient is multiplied by (``grad_norm``'s second result).  Parameters
-    are float32 or bfloat16, gradients of the same dtype, all contiguous and on one device.
+    are float32 or bfloat16, gradients of the same dtype, all contiguous and on one device, parameters
+    and states no negated views.
     8-bit states and bfloat16 parameters are rounded stochastically, by a pure function of
     ``seed`` (an int of up to 64 bits), the tensor's step, its place in the list and the
     element: the same call gives the same bits.  Tensors must not overlap.  Step counts,
@@ -259,12 +265,16 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
     if not n:
         return
     dev, at = params[0].device, params[0].get_device()
-    launches, seen = {}, set()
+    launches, seen, keep = {}, set(), []
     for k, (p, g, st) in enumerate(zip(params, grads, states)):
         dt = p.dtype
         if at < 0 or dt not in _C.DTYPES or g.dtype is not dt or p.get_device() != at or g.get_device() != at or \
-                g.shape != p.shape or not (p.is_contiguous() and g.is_contiguous()):
+                not p.is_same_size(g) or not (p.is_contiguous() and g.is_contiguous()) or \
+                dt is _F32 and p.is_neg():
             _adamw_refuse(p, g, dev)
+        if dt is _F32 and g.is_neg():  # as a conjugated complex number's imaginary part leaves it: its bytes are not its values
+            g = g.resolve_neg()
+            keep.append(g)  # until the launch
         size = p.numel()
         bits, m, v, ms, vs = _state_ptrs(st, p, size, "adamw_step")
         if not size:
@@ -281,6 +291,8 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
     with _on(dev):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("adamw_step: step counts and rates are host values; not for graph capture")
+        if grad_scale is not None:
+            grad_scale = grad_scale.resolve_neg()
         stream, scale = _C._stream(dev), None if grad_scale is None else grad_scale.data_ptr()
         seed &= 0xFFFFFFFFFFFFFFFF
         tables = [(kind, struct.pack("7q2d2i" * (len(segs) // 11), *segs), len(segs) // 11)  # gsr_adamw_segment
@@ -431,7 +443,7 @@ def select_rows(score: torch.Tensor, budget: int, protect: torch.Tensor = None) 
                            f"{tuple(protect.shape)} on {protect.device}")
     dev = score.device
     with _on(dev):
-        s = score.contiguous()
+        s = score.resolve_neg().contiguous()
         pr = None if protect is None else protect.contiguous()
         rows = torch.empty(min(budget, P), dtype=torch.int64, device=dev)
         if rows.numel():
@@ -484,7 +496,7 @@ def take_rows(tensors, rows: torch.Tensor, states=None):
         plain = tensors
         for st in states or ():
             m = st["exp_avg"]
-            bits, mp, vp, msp, vsp = _state_ptrs(st, m, m.numel(), "take_rows")
+            bits, mp, vp, msp, vsp = _state_ptrs(st, m, m.numel(), "take_rows", raw=False)
             got = {"step": st["step"]}
             new_states.append(got)
             if bits == 32:

@@ -738,3 +738,73 @@ def test_state_dict_round_trip(dev, bits, tmp_path):
     bad["state"][0]["exp_avg"] = bad["state"][0]["exp_avg"][:5]
     with pytest.raises(RuntimeError, match="exp_avg"):
         ob.load_state_dict(bad)
+
+
+# ------------------------------------------------------------------ GPU: values that are not their bytes
+def _negated(x):
+    """x as a view of -x's bytes, as the backward of a conjugated complex number leaves it."""
+    return torch._neg_view(-x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_step_takes_negated_gradients_and_scale(dev, bits):
+    import train_ops
+
+    for n in (1, 777):
+        p, g, m, v = _inputs(n, n + 3)
+        assert g.any()
+        got = []
+        for neg_grad, neg_scale in ((False, False), (True, False), (False, True)):
+            P, G, scale = p.to(dev), g.to(dev), torch.tensor(0.25, device=dev)
+            G, scale = _negated(G) if neg_grad else G, _negated(scale) if neg_scale else scale
+            assert G.is_contiguous() and G.is_neg() == neg_grad and scale.is_neg() == neg_scale
+            st = {"step": 3, "exp_avg": m.to(dev), "exp_avg_sq": v.to(dev)} if bits == 32 else _state8(m, v, dev)
+            train_ops.adamw_step([P], [G], [st], 0.01, grad_scale=scale)
+            got.append([P] + [x.view(torch.uint8) for k, x in st.items() if k != "step"])
+        for other in got[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+
+
+@pytest.mark.gpu
+def test_optimiser_takes_the_gradient_that_a_complex_loss_leaves(dev):
+    """b.grad of one element is contiguous and a negated view."""
+    import train_ops
+
+    def loss(a, b):
+        return (torch.complex(a, b).conj() * torch.tensor([0.3 - 0.7j], device=dev)).real.sum()
+
+    new = lambda: [torch.ones(1, device=dev, requires_grad=True) for _ in range(2)]  # noqa: E731
+    pa, pb = new(), new()
+    opt = train_ops.FusedAdamW([{"params": pa, "lr": 0.1}], eps=1e-8, max_norm=1.0)
+    ref = torch.optim.AdamW(pb, lr=0.1, eps=1e-8, weight_decay=0.0)
+    for _ in range(3):
+        loss(*pa).backward()
+        loss(*pb).backward()
+        assert pa[1].grad.is_neg() and pa[1].grad.is_contiguous()
+        for q in pb:
+            q.grad = q.grad.resolve_neg()  # torch's list operations refuse it
+        opt.step()
+        torch.nn.utils.clip_grad_norm_(pb, 1.0)
+        ref.step()
+        opt.zero_grad()
+        ref.zero_grad()
+    # three steps of about 14 roundings each, of values of order 1
+    torch.testing.assert_close(torch.cat(pa), torch.cat(pb), rtol=0, atol=3 * 14 * U)
+
+
+@pytest.mark.gpu
+def test_step_refuses_negated_parameters_and_states(dev):
+    import train_ops
+
+    p, g = torch.randn(6, device=dev), torch.randn(6, device=dev)
+    for kw, msg in ((dict(params=[_negated(p)]), "negated"), (dict(key="exp_avg"), "exp_avg"),
+                    (dict(key="exp_avg_sq"), "exp_avg_sq")):
+        st = train_ops.adamw_state(p)
+        if "key" in kw:
+            st[kw["key"]] = _negated(st[kw["key"]])
+        q = kw.get("params", [p])
+        before = q[0].clone()
+        with pytest.raises(RuntimeError, match=msg):
+            train_ops.adamw_step(q, [g], [st], 0.1)
+        assert torch.equal(q[0], before) and st["step"] == 0

@@ -502,3 +502,23 @@ def test_prune_needs_the_optimiser_that_moves_states(dev):
     st = train_step.TrainState(g, 1.0, fused=True, state_bits=32)
     with pytest.raises(RuntimeError, match="scores"):
         st.prune_to_budget(g, torch.zeros(9, device=dev), 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("P", [1000, 20_000])
+def test_select_rows_of_a_negated_view(dev, P):
+    import train_ops
+
+    s = torch.randn(P, generator=torch.Generator().manual_seed(P))
+    got = train_ops.select_rows(torch._neg_view(-s.to(dev)), P // 3)
+    assert torch.equal(got.cpu(), torch.tensor(_select(s, P // 3)))
+
+
+@pytest.mark.gpu
+def test_take_rows_of_negated_states(dev):
+    import train_ops
+
+    m, rows = torch.randn(50, 3, device=dev), torch.tensor([7, -1, 49], device=dev)
+    st = {"step": 1, "exp_avg": torch._neg_view(-m), "exp_avg_sq": m * m}
+    _, (got,) = train_ops.take_rows([], rows, [st])
+    assert torch.equal(got["exp_avg"][[0, 2]], m[[7, 49]]) and not got["exp_avg"][1].any()
