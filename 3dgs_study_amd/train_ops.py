@@ -104,7 +104,7 @@ class FusedAdam:
         rejected call leaves no parameter's state advanced."""
         lib = _C.load_library()
         segs = (_C.GsrAdamSegment * _C.ADAM_MAX_SEGS)()
-        todo = []
+        todo, grads = [], []
         for g in self.param_groups:
             for p in g["params"]:
                 if p.grad is None:
@@ -112,7 +112,10 @@ class FusedAdam:
                 _cuda(p, "FusedAdam")
                 if not (p.is_contiguous() and p.grad.is_contiguous()):
                     raise RuntimeError("FusedAdam: parameters and gradients must be contiguous")
+                if p.is_neg():
+                    raise RuntimeError("FusedAdam: parameters must not be negated views")
                 todo.append((g, p))
+                grads.append(p.grad.resolve_neg())  # a complex number's backward may leave a negated view
         if len(todo) > _C.ADAM_MAX_SEGS:
             raise RuntimeError(f"FusedAdam: at most {_C.ADAM_MAX_SEGS} tensors per launch")
         steps = {self.state[p]["step"] if p in self.state else 0 for _, p in todo}
@@ -126,7 +129,7 @@ class FusedAdam:
             if st is None:
                 st = self.state[p] = {"step": 0, "exp_avg": torch.zeros_like(p), "exp_avg_sq": torch.zeros_like(p)}
             st["step"] = step
-            segs[n] = _C.GsrAdamSegment(p.data_ptr(), p.grad.data_ptr(), st["exp_avg"].data_ptr(),
+            segs[n] = _C.GsrAdamSegment(p.data_ptr(), grads[n].data_ptr(), st["exp_avg"].data_ptr(),
                                         st["exp_avg_sq"].data_ptr(), p.numel(), float(g["lr"]))
         _C._check(lib.gsr_adam_step(segs, len(todo), step, self.betas[0], self.betas[1], self.eps,
                                     _C._stream(todo[0][1].device)), "gsr_adam_step")

@@ -189,3 +189,34 @@ def test_full_train_step_fused_matches_torch(dev):
     a, b = out[True][2].xyz_gradient_accum, out[False][2].xyz_gradient_accum
     off = (a - b).abs() > 1e-4 * b.abs() + 1e-9
     assert float(off.float().mean()) < 0.01, float(off.float().mean())
+
+
+@pytest.mark.gpu
+def test_fused_adam_takes_the_gradient_that_a_complex_loss_leaves(dev):
+    """b.grad of one element is contiguous and a negated view: its values are not its bytes."""
+    import train_ops
+
+    def loss(a, b):
+        return (torch.complex(a, b).conj() * torch.tensor([0.3 - 0.7j], device=dev)).real.sum()
+
+    new = lambda: [torch.ones(1, device=dev, requires_grad=True) for _ in range(2)]  # noqa: E731
+    pa, pb = new(), new()
+    opt = train_ops.FusedAdam([{"params": pa, "lr": 0.1}], eps=1e-8)
+    ref = torch.optim.Adam(pb, lr=0.1, eps=1e-8)
+    for _ in range(3):
+        loss(*pa).backward()
+        loss(*pb).backward()
+        assert pa[1].grad.is_neg() and pa[1].grad.is_contiguous()
+        for q in pb:
+            q.grad = q.grad.resolve_neg()  # torch's list operations refuse it
+        opt.step()
+        ref.step()
+        opt.zero_grad()
+        ref.zero_grad()
+    # three steps of at most 14 roundings each, of values of order 1: 3 * 14 * 2^-24
+    torch.testing.assert_close(torch.cat(pa), torch.cat(pb), rtol=0, atol=42 * 2.0 ** -24)
+    opt = train_ops.FusedAdam([{"params": [torch._neg_view(torch.ones(3, device=dev))], "lr": 0.1}])
+    opt.param_groups[0]["params"][0].grad = torch.ones(3, device=dev)
+    with pytest.raises(RuntimeError, match="negated"):
+        opt.step()
+    assert not opt.state
