@@ -242,11 +242,20 @@ def _adamw_refuse(p: torch.Tensor, g: torch.Tensor, dev):
     raise RuntimeError("adamw_step: parameters and gradients must be contiguous")
 
 
+_ADAMW_MOST = 1 << 33  # elements of a tensor (include/gsr.h gsr_adamw_step)
+
+
+def _adamw_refuse_count(count, size: int):
+    if count is None or count < 0:
+        raise RuntimeError(f"adamw_step: a state's step must be a count >= 0 (got {count!r})")
+    raise RuntimeError(f"adamw_step: a tensor's size must be at most 2^33 elements (got {size})")
+
+
 def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), eps: float = 1e-15,
                grad_scale: torch.Tensor = None, seed: int = 0):
-    """One AdamW step in place over lists of tensors: parameters, their gradients and their
-    states (``adamw_state``; 32- and 8-bit ones may be mixed), in one launch for up to 40
-    tensors of a dtype and state width.
+    """One AdamW step in place over lists of tensors of up to 2^33 elements: parameters, their
+    gradients and their states (``adamw_state``; 32- and 8-bit ones may be mixed), in one launch
+    for up to 40 tensors of a dtype and state width.
 
     ``lr`` and ``weight_decay``: a number, or one per tensor.  Each state's ``step`` counts
     its own tensor's steps and is advanced by one.  ``grad_scale``: a float32 scalar on the
@@ -280,6 +289,9 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
             keep.append(g)  # until the launch
         size = p.numel()
         bits, m, v, ms, vs = _state_ptrs(st, p, size, "adamw_step")
+        count = st.get("step")
+        if count is None or count < 0 or size > _ADAMW_MOST:  # what the library would refuse of a later launch
+            _adamw_refuse_count(count, size)
         if not size:
             continue
         addr = p.data_ptr()
@@ -287,7 +299,7 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
             raise RuntimeError("adamw_step: a parameter or state appears twice")
         seen.update((addr, m))
         launches.setdefault((dt, bits), []).extend((addr, g.data_ptr(), m, v, ms, vs, size, lrs[k], wds[k],
-                                                    st["step"] + 1, k))
+                                                    count + 1, k))
     if grad_scale is not None and (grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1 or
                                    grad_scale.device != dev):
         raise RuntimeError(f"adamw_step: grad_scale must be a float32 scalar on {dev}")

@@ -808,3 +808,31 @@ def test_step_refuses_negated_parameters_and_states(dev):
         with pytest.raises(RuntimeError, match=msg):
             train_ops.adamw_step(q, [g], [st], 0.1)
         assert torch.equal(q[0], before) and st["step"] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["negative", "missing", "large"])
+def test_step_a_refusal_of_a_later_kind_comes_before_the_first_launch(dev, what):
+    """Lists whose tensors go out in several launches: what the second would refuse stops all."""
+    import train_ops
+
+    p, q = torch.ones(5, device=dev), torch.ones(5, device=dev)
+    states = [train_ops.adamw_state(p), train_ops.adamw_state(q, 8)]
+    grads = [torch.ones_like(p), torch.ones_like(q)]
+    if what == "negative":
+        states[1]["step"] = -1
+    elif what == "missing":  # of an empty tensor, which goes out in no launch
+        q, grads[1] = q[:0], grads[1][:0]
+        states[1] = train_ops.adamw_state(q, 8)
+        del states[1]["step"]
+    else:  # never touched: the gradient is the parameter itself
+        q = torch.empty((1 << 33) + 1, dtype=torch.bfloat16, device=dev)
+        grads[1] = q
+        codes = lambda: torch.empty(q.numel(), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)  # noqa: E731
+        scale = lambda: torch.empty((1 << 27) + 1, dtype=torch.uint8, device=dev).view(torch.float8_e8m0fnu)  # noqa: E731
+        states[1] = {"step": 0, "exp_avg": codes(), "exp_rms": codes(), "exp_avg_scale": scale(), "exp_rms_scale": scale()}
+    count = states[1].get("step")
+    with pytest.raises(RuntimeError, match="size" if what == "large" else "step"):
+        train_ops.adamw_step([p, q], grads, states, 0.1)
+    assert torch.equal(p, torch.ones_like(p)) and not states[0]["exp_avg"].any() and not states[0]["exp_avg_sq"].any()
+    assert states[0]["step"] == 0 and states[1].get("step") == count
