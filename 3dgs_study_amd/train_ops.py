@@ -277,7 +277,7 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
     if not n:
         return
     dev, at = params[0].device, params[0].get_device()
-    launches, seen, keep = {}, set(), []
+    launches, seen, written, keep = {}, set(), 0, []
     for k, (p, g, st) in enumerate(zip(params, grads, states)):
         dt = p.dtype
         if at < 0 or dt not in _C.DTYPES or g.dtype is not dt or p.get_device() != at or g.get_device() != at or \
@@ -295,9 +295,10 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
         if not size:
             continue
         addr = p.data_ptr()
-        if addr in seen or m in seen:
-            raise RuntimeError("adamw_step: a parameter or state appears twice")
-        seen.update((addr, m))
+        written += 3 if bits == 32 else 5
+        seen.update((addr, m, v) if bits == 32 else (addr, m, v, ms, vs))
+        if len(seen) != written:
+            raise RuntimeError("adamw_step: a parameter or a part of a state appears twice")
         launches.setdefault((dt, bits), []).extend((addr, g.data_ptr(), m, v, ms, vs, size, lrs[k], wds[k],
                                                     count + 1, k))
     if grad_scale is not None and (grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1 or

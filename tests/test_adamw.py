@@ -836,3 +836,31 @@ def test_step_a_refusal_of_a_later_kind_comes_before_the_first_launch(dev, what)
         train_ops.adamw_step([p, q], grads, states, 0.1)
     assert torch.equal(p, torch.ones_like(p)) and not states[0]["exp_avg"].any() and not states[0]["exp_avg_sq"].any()
     assert states[0]["step"] == 0 and states[1].get("step") == count
+
+
+@pytest.mark.gpu
+def test_step_refuses_states_that_share_any_buffer(dev):
+    """Every buffer that the step writes: a shared one would be read and written by two workgroups at once."""
+    import train_ops
+
+    ps = [torch.ones(100, device=dev), torch.ones(100, device=dev)]
+    gs = [torch.ones(100, device=dev)] * 2  # gradients are only read
+    for bits, keys in ((32, ("exp_avg", "exp_avg_sq")), (8, ("exp_avg", "exp_avg_scale", "exp_rms", "exp_rms_scale"))):
+        for key in keys:
+            st = [train_ops.adamw_state(p, bits) for p in ps]
+            st[1][key] = st[0][key]
+            with pytest.raises(RuntimeError, match="twice"):
+                train_ops.adamw_step(ps, gs, st, 0.1)
+            assert st[0]["step"] == st[1]["step"] == 0
+        one = train_ops.adamw_state(ps[0], bits)
+        one[keys[-1]] = one[keys[-1] if bits == 32 else "exp_avg_scale"]
+        if bits == 32:
+            one["exp_avg_sq"] = one["exp_avg"]
+        with pytest.raises(RuntimeError, match="twice"):
+            train_ops.adamw_step(ps[:1], gs[:1], [one], 0.1)
+    st = train_ops.adamw_state(ps[0])
+    with pytest.raises(RuntimeError, match="twice"):  # a state that is another tensor's parameter
+        train_ops.adamw_step(ps, gs, [{**st, "exp_avg_sq": ps[1]}, train_ops.adamw_state(ps[1])], 0.1)
+    assert all(torch.equal(p, torch.ones_like(p)) for p in ps)
+    train_ops.adamw_step(ps, gs, [train_ops.adamw_state(p) for p in ps], 0.1)  # a shared gradient is in order
+    assert torch.equal(ps[0], ps[1])
