@@ -348,10 +348,27 @@ def grad_norm(grads, max_norm: float = math.inf):
     return out.unbind()
 
 
+def _adamw_options(groups) -> tuple:
+    """(betas, eps) of the param groups, which share them; what a step would not do is refused."""
+    got = set()
+    for g in groups:
+        for k in ("amsgrad", "maximize"):
+            if g.get(k):
+                raise ValueError(f"FusedAdamW: {k} is not implemented")
+        if g["weight_decay"] and not g.get("decoupled_weight_decay", True):
+            raise ValueError("FusedAdamW: weight decay is decoupled (a checkpoint of torch.optim.Adam's is not)")
+        b1, b2 = g["betas"]
+        got.add(((float(b1), float(b2)), float(g["eps"])))
+    if len(got) > 1:
+        raise ValueError(f"FusedAdamW: all groups have the same betas and eps (got {sorted(got)})")
+    return got.pop() if got else None
+
+
 class FusedAdamW:
     """AdamW over param groups (``params``, ``lr``, optionally ``weight_decay``, ``name``), with
     the moments in 32 bits or in 8 (``state_bits``), and gradients clipped to a global norm of
-    ``max_norm`` (None: not clipped).  ``state[p]`` is ``adamw_state``'s dict: with 32 bits the
+    ``max_norm`` (None: not clipped).  ``betas`` and ``eps`` stand in the groups, as torch's do, with
+    the same values in all of them.  ``state[p]`` is ``adamw_state``'s dict: with 32 bits the
     names that code for torch's optimizer expects.  After each step ``grad_norm`` holds the
     norm before clipping (a device scalar; None without clipping)."""
 
@@ -363,15 +380,26 @@ class FusedAdamW:
         for g in self.param_groups:
             g.setdefault("lr", lr)
             g.setdefault("weight_decay", weight_decay)
-        self.betas, self.eps, self.state_bits, self.max_norm, self.seed = betas, eps, state_bits, max_norm, seed
+            g.setdefault("betas", tuple(betas))
+            g.setdefault("eps", eps)
+        _adamw_options(self.param_groups)
+        self.state_bits, self.max_norm, self.seed = state_bits, max_norm, seed
         self.state = {}
         self.grad_norm = None
+
+    def _set_option(self, key, value):
+        for g in self.param_groups:
+            g[key] = value
+
+    betas = property(lambda self: _adamw_options(self.param_groups)[0], lambda self, b: self._set_option("betas", tuple(b)))
+    eps = property(lambda self: _adamw_options(self.param_groups)[1], lambda self, e: self._set_option("eps", e))
 
     @torch.no_grad()
     def step(self):
         todo = [(g, p) for g in self.param_groups for p in g["params"] if p.grad is not None]
         if not todo:
             return
+        betas, eps = _adamw_options(self.param_groups)
         params = [p for _, p in todo]
         grads = [p.grad for p in params]
         states = [self.state[p] if p in self.state else adamw_state(p, self.state_bits) for p in params]
@@ -379,7 +407,7 @@ class FusedAdamW:
         if self.max_norm is not None:
             norm, scale = grad_norm(grads, self.max_norm)
         adamw_step(params, grads, states, [g["lr"] for g, _ in todo], [g["weight_decay"] for g, _ in todo],
-                   self.betas, self.eps, scale, self.seed)
+                   betas, eps, scale, self.seed)
         self.grad_norm = norm
         self.state.update(zip(params, states))
 
@@ -387,20 +415,28 @@ class FusedAdamW:
 
     def state_dict(self) -> dict:
         """{"state": {place: state}, "param_groups": [...]} in torch.optim's form (the tensors
-        themselves, not copies): place counts the parameters through the groups."""
+        themselves, not copies): place counts the parameters through the groups.  Beside them
+        "seed", "max_norm" and "state_bits", so that a loaded optimiser continues bit for bit."""
         params = [p for g in self.param_groups for p in g["params"]]
         groups, at = [], 0
         for g in self.param_groups:
             groups.append({**g, "params": list(range(at, at + len(g["params"])))})
             at += len(g["params"])
         return {"state": {k: dict(self.state[p]) for k, p in enumerate(params) if p in self.state},
-                "param_groups": groups}
+                "param_groups": groups, "seed": self.seed, "max_norm": self.max_norm, "state_bits": self.state_bits}
 
     def load_state_dict(self, d: dict):
-        """Takes over ``state_dict``'s states (copied to their parameters' device) and the
-        groups' options.  States of either width are taken as they are."""
+        """Takes over ``state_dict``'s states (copied to their parameters' device), the groups' options
+        (betas and eps among them) and what stands beside them; a dict of torch.optim.AdamW, which has
+        no such things, leaves those as they are.  States of either width are taken as they are.
+        Options that a step would not follow (amsgrad, maximize, betas by group) are refused."""
         if [len(g["params"]) for g in d["param_groups"]] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("FusedAdamW.load_state_dict: other param groups")
+        groups = [{**g, **{n: x for n, x in h.items() if n != "params"}} for g, h in zip(self.param_groups, d["param_groups"])]
+        _adamw_options(groups)
+        state_bits = d.get("state_bits", self.state_bits)
+        if state_bits not in _KEYS:
+            raise ValueError(f"FusedAdamW.load_state_dict: state_bits must be 32 or 8 (got {state_bits})")
         params = [p for g in self.param_groups for p in g["params"]]
         state = {}
         for k, st in d["state"].items():
@@ -409,9 +445,10 @@ class FusedAdamW:
             st["step"] = int(st["step"])
             _state_ptrs(st, p, p.numel(), "FusedAdamW.load_state_dict")
             state[p] = st
-        self.state = state
-        for g, h in zip(self.param_groups, d["param_groups"]):
-            g.update({n: x for n, x in h.items() if n != "params"})
+        self.state, self.state_bits = state, state_bits
+        self.seed, self.max_norm = d.get("seed", self.seed), d.get("max_norm", self.max_norm)
+        for g, h in zip(self.param_groups, groups):
+            g.update(h)
 
     @torch.no_grad()
     def take_rows(self, rows: torch.Tensor, fresh: torch.Tensor = None) -> list:

@@ -864,3 +864,86 @@ def test_step_refuses_states_that_share_any_buffer(dev):
     assert all(torch.equal(p, torch.ones_like(p)) for p in ps)
     train_ops.adamw_step(ps, gs, [train_ops.adamw_state(p) for p in ps], 0.1)  # a shared gradient is in order
     assert torch.equal(ps[0], ps[1])
+
+
+def _adamw_on_cpu(**kw):
+    import train_ops
+
+    ps = [torch.ones(3, requires_grad=True), torch.ones(2, requires_grad=True)]
+    return ps, train_ops.FusedAdamW([{"params": ps[:1], "lr": 0.1}, {"params": ps[1:]}], **kw)
+
+
+def test_load_state_dict_takes_the_hyperparameters_of_a_torch_checkpoint():
+    _, opt = _adamw_on_cpu(seed=4, max_norm=2.0)
+    qs = [torch.ones(3, requires_grad=True), torch.ones(2, requires_grad=True)]
+    ref = torch.optim.AdamW([{"params": qs[:1]}, {"params": qs[1:]}], lr=0.3, betas=(0.5, 0.6), eps=1e-8)
+    for q in qs:
+        q.grad = torch.ones_like(q)
+    ref.step()
+    opt.load_state_dict(ref.state_dict())
+    assert opt.betas == (0.5, 0.6) and opt.eps == 1e-8
+    assert opt.param_groups[0]["lr"] == 0.3 and opt.param_groups[0]["weight_decay"] == 0.01
+    assert opt.seed == 4 and opt.max_norm == 2.0  # not in such a checkpoint: as constructed
+    assert all(s["step"] == 1 for s in opt.state.values()) and len(opt.state) == 2
+
+
+def test_state_dict_holds_all_that_a_step_depends_on():
+    ps, a = _adamw_on_cpu(betas=(0.8, 0.9), eps=1e-6, seed=7, max_norm=3.0, state_bits=8, weight_decay=0.1)
+    _, b = _adamw_on_cpu()
+    b.load_state_dict(a.state_dict())
+    assert (b.betas, b.eps, b.seed, b.max_norm, b.state_bits) == ((0.8, 0.9), 1e-6, 7, 3.0, 8)
+    assert [g["weight_decay"] for g in b.param_groups] == [0.1, 0.1]
+    # torch's own optimiser takes it too
+    ref = torch.optim.AdamW([{"params": ps[:1]}, {"params": ps[1:]}], lr=0.3)
+    ref.load_state_dict(a.state_dict())
+    assert ref.param_groups[0]["betas"] == (0.8, 0.9) and ref.param_groups[0]["eps"] == 1e-6
+    b.betas, b.eps = (0.7, 0.95), 1e-9
+    assert all(g["betas"] == (0.7, 0.95) and g["eps"] == 1e-9 for g in b.param_groups)
+
+
+@pytest.mark.parametrize("change, msg", [(dict(amsgrad=True), "amsgrad"), (dict(maximize=True), "maximize"),
+                                         (dict(betas=(0.5, 0.9)), "betas"), (dict(eps=1e-3), "eps"),
+                                         (dict(decoupled_weight_decay=False, weight_decay=0.1), "decoupled")])
+def test_options_that_a_step_would_ignore_are_refused(change, msg):
+    import train_ops
+
+    ps, opt = _adamw_on_cpu()
+    with pytest.raises(ValueError, match=msg):  # at construction
+        train_ops.FusedAdamW([{"params": ps[:1]}, {"params": ps[1:], **change}])
+    d = opt.state_dict()
+    d["param_groups"][1].update(change)
+    d["param_groups"][0]["lr"] = 9.0
+    d["seed"] = 5
+    d["state"] = {0: {**train_ops.adamw_state(ps[0]), "step": 3}}
+    with pytest.raises(ValueError, match=msg):  # on loading, which then changes nothing
+        opt.load_state_dict(d)
+    assert opt.param_groups[0]["lr"] == 0.1 and opt.seed == 0 and not opt.state
+    opt.param_groups[1].update(change)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match=msg):  # and at the step
+        opt.step()
+
+
+@pytest.mark.gpu
+def test_step_after_loading_goes_by_the_checkpoints_betas_and_eps(dev):
+    """A torch.optim.AdamW checkpoint with its own betas and eps, continued by both."""
+    import train_ops
+
+    gen = torch.Generator().manual_seed(3)
+    base, grads = torch.randn(500, generator=gen), [torch.randn(500, generator=gen).to(dev) for _ in range(4)]
+    q = base.clone().to(dev).requires_grad_(True)
+    ref = torch.optim.AdamW([q], lr=0.01, betas=(0.5, 0.6), eps=1e-3, weight_decay=0.0)
+    for g in grads[:2]:
+        q.grad = g
+        ref.step()
+    p = q.detach().clone().requires_grad_(True)
+    opt = train_ops.FusedAdamW([{"params": [p]}])
+    opt.load_state_dict(ref.state_dict())
+    for g in grads[2:]:
+        p.grad = q.grad = g
+        opt.step()
+        ref.step()
+    # two steps: 3 roundings of p each and 12 of updates of at most about 2 lr; moments of order 1
+    torch.testing.assert_close(p, q, rtol=8 * U, atol=2 * 12 * U * 0.02 + 8 * U * 0.02)
+    torch.testing.assert_close(opt.state[p]["exp_avg_sq"], ref.state[q]["exp_avg_sq"], rtol=12 * U, atol=0)
