@@ -313,10 +313,11 @@ class TrainState:
     schedule and the densification statistics (:565-581).  ``fused`` swaps torch's
     Adam and statistics for the HIP kernels of train_ops.py; with it, any of
     ``state_bits`` (32 or 8: the moments' width), ``weight_decay`` and ``max_norm`` (global
-    gradient norm to clip to) takes train_ops.FusedAdamW instead of FusedAdam."""
+    gradient norm to clip to) takes train_ops.FusedAdamW instead of FusedAdam; ``seed`` is its
+    rounding's."""
 
     def __init__(self, g, spatial_lr_scale: float, fused: bool = False, opt: dict = OPT, state_bits: int = None,
-                 weight_decay: float = 0.0, max_norm: float = None):
+                 weight_decay: float = 0.0, max_norm: float = None, seed: int = 0):
         import train_ops
 
         self.opt, self.fused = opt, fused
@@ -331,9 +332,12 @@ class TrainState:
         adamw = state_bits is not None or weight_decay or max_norm is not None
         if adamw and not fused:
             raise ValueError("TrainState: state_bits, weight_decay and max_norm need fused=True")
+        if seed and not adamw:
+            raise ValueError("TrainState: seed needs state_bits, weight_decay or max_norm (nothing else is rounded at random)")
         if adamw:
             self.optimizer = train_ops.FusedAdamW(groups, lr=0.0, eps=1e-15, weight_decay=weight_decay,
-                                                  state_bits=state_bits or 32, max_norm=max_norm)
+                                                  state_bits=32 if state_bits is None else state_bits,
+                                                  max_norm=max_norm, seed=seed)
         elif fused:
             self.optimizer = train_ops.FusedAdam(groups, lr=0.0, eps=1e-15)
         else:

@@ -947,3 +947,19 @@ def test_step_after_loading_goes_by_the_checkpoints_betas_and_eps(dev):
     # two steps: 3 roundings of p each and 12 of updates of at most about 2 lr; moments of order 1
     torch.testing.assert_close(p, q, rtol=8 * U, atol=2 * 12 * U * 0.02 + 8 * U * 0.02)
     torch.testing.assert_close(opt.state[p]["exp_avg_sq"], ref.state[q]["exp_avg_sq"], rtol=12 * U, atol=0)
+
+
+def test_train_state_adamw_options():
+    import synthetic
+    import train_ops
+    import train_step
+
+    g = synthetic.make_gaussians(4, 1)
+    with pytest.raises(ValueError, match="state_bits"):
+        train_step.TrainState(g, 1.0, fused=True, state_bits=0)
+    opt = train_step.TrainState(g, 1.0, fused=True, state_bits=8, seed=11).optimizer
+    assert isinstance(opt, train_ops.FusedAdamW) and opt.seed == 11 and opt.state_bits == 8
+    assert train_step.TrainState(g, 1.0, fused=True, max_norm=1.0).optimizer.state_bits == 32
+    for fused in (False, True):
+        with pytest.raises(ValueError, match="seed"):  # of nothing that would use it
+            train_step.TrainState(g, 1.0, fused=fused, seed=11)
