@@ -314,10 +314,12 @@ class TrainState:
     Adam and statistics for the HIP kernels of train_ops.py; with it, any of
     ``state_bits`` (32 or 8: the moments' width), ``weight_decay`` and ``max_norm`` (global
     gradient norm to clip to) takes train_ops.FusedAdamW instead of FusedAdam; ``seed`` is its
-    rounding's."""
+    rounding's.  ``weight_decay``: a number for all six groups, which draws positions to the
+    origin, log scales to 0 and quaternions to nothing too, or {group's name: number} with 0 for
+    the others."""
 
     def __init__(self, g, spatial_lr_scale: float, fused: bool = False, opt: dict = OPT, state_bits: int = None,
-                 weight_decay: float = 0.0, max_norm: float = None, seed: int = 0):
+                 weight_decay: float | dict = 0.0, max_norm: float = None, seed: int = 0):
         import train_ops
 
         self.opt, self.fused = opt, fused
@@ -334,6 +336,13 @@ class TrainState:
             raise ValueError("TrainState: state_bits, weight_decay and max_norm need fused=True")
         if seed and not adamw:
             raise ValueError("TrainState: seed needs state_bits, weight_decay or max_norm (nothing else is rounded at random)")
+        if isinstance(weight_decay, dict):
+            unknown = set(weight_decay) - {group["name"] for group in groups}
+            if unknown:
+                raise ValueError(f"TrainState: weight_decay for {sorted(unknown)}, which are no groups")
+            for group in groups:
+                group["weight_decay"] = weight_decay.get(group["name"], 0.0)
+            weight_decay = 0.0
         if adamw:
             self.optimizer = train_ops.FusedAdamW(groups, lr=0.0, eps=1e-15, weight_decay=weight_decay,
                                                   state_bits=32 if state_bits is None else state_bits,

@@ -963,3 +963,18 @@ def test_train_state_adamw_options():
     for fused in (False, True):
         with pytest.raises(ValueError, match="seed"):  # of nothing that would use it
             train_step.TrainState(g, 1.0, fused=fused, seed=11)
+
+
+def test_train_state_decays_the_groups_that_are_named():
+    import synthetic
+    import train_step
+
+    g = synthetic.make_gaussians(4, 1)
+    decay = lambda wd: [x["weight_decay"] for x in  # noqa: E731
+                        train_step.TrainState(g, 1.0, fused=True, weight_decay=wd).optimizer.param_groups]
+    assert decay(0.1) == [0.1] * 6
+    assert decay({"f_rest": 0.1, "opacity": 0.2}) == [0.0, 0.0, 0.1, 0.2, 0.0, 0.0]
+    with pytest.raises(ValueError, match="positions"):
+        train_step.TrainState(g, 1.0, fused=True, weight_decay={"positions": 0.1})
+    with pytest.raises(ValueError, match="fused"):
+        train_step.TrainState(g, 1.0, weight_decay={"f_rest": 0.1})
