@@ -869,3 +869,26 @@ def reduce_densification_stats(xyz_gradient_accum: torch.Tensor, denom: torch.Te
     w2.wait()
     n = xyz_gradient_accum.numel()
     return both[:n].view_as(xyz_gradient_accum), both[n:].view_as(denom), mx
+
+
+@torch.no_grad()
+def reduce_blend_weight(score: torch.Tensor, protect: torch.Tensor = None, group=None, force: bool = False):
+    """The ranks' accumulated blending weights (train_step.accumulate_blend_weight, each of its own
+    views) combined for an eviction to a budget: the SUM of the scores, and the rows that any
+    rank protects, in one all-reduce, so every rank keeps the same rows and the replicas stay
+    identical.  ``score``: float32 [P] or [P,1]; ``protect``: P bools, or None (on some ranks, or
+    all).  Returns copies (score, protect) and leaves the rank's own as they are; without a
+    process group of more than one rank, (a copy of the score, protect)."""
+    P = score.numel()
+    if score.dtype is not torch.float32:
+        raise RuntimeError(f"reduce_blend_weight: float32 scores expected, got {score.dtype}")
+    if protect is not None and (protect.dtype is not torch.bool or protect.numel() != P):
+        raise RuntimeError(f"reduce_blend_weight: protect must be {P} bools, got {protect.dtype} {tuple(protect.shape)}")
+    if not (dist.is_initialized() and (dist.get_world_size(group) > 1 or force)):
+        return score.clone(), protect
+    both = torch.zeros(2 * P, dtype=torch.float32, device=score.device)  # the same size with and without protect
+    both[:P] = score.reshape(-1)
+    if protect is not None:
+        both[P:] = protect.reshape(-1)
+    dist.all_reduce(both, op=dist.ReduceOp.SUM, group=group)
+    return both[:P].view_as(score), both[P:] > 0

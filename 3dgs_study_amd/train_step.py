@@ -367,19 +367,27 @@ class TrainState:
                 return group["lr"]
 
     @torch.no_grad()
-    def prune_to_budget(self, g, score: torch.Tensor, budget: int, protect: torch.Tensor = None) -> torch.Tensor:
+    def prune_to_budget(self, g, score: torch.Tensor, budget: int, protect: torch.Tensor = None,
+                        group=None) -> torch.Tensor:
         """Evicts the Gaussians of the smallest ``score`` ([P]: accumulate_blend_weight over
         the views) so that ``budget`` stay (train_ops.select_rows: ties, NaN, ``protect``): the
         model's six parameters, their optimiser states and the densification statistics are
         replaced by the kept rows, in order.  Returns those rows (int64); the caller's own
         per-Gaussian tensors follow with train_ops.take_rows; what is bound to the old
-        parameters (a gradient reducer, a captured unit) is made anew.  Needs FusedAdamW."""
+        parameters (a gradient reducer, a captured unit) is made anew.  Needs FusedAdamW.
+
+        View-parallel: with more than one rank in ``group`` (None: all ranks of
+        torch.distributed) every rank calls this with the weight of its own views; the rows that stay
+        are those that any rank protects and those of the largest sums (multiview.reduce_blend_weight),
+        the same on every rank.  Ranks that train models of their own pass a group of one."""
+        import multiview
         import train_ops
 
         if not isinstance(self.optimizer, train_ops.FusedAdamW):
             raise RuntimeError("prune_to_budget: needs a TrainState with FusedAdamW (state_bits=)")
         if score.shape[0] != g.xyz.shape[0]:
             raise RuntimeError(f"prune_to_budget: {score.shape[0]} scores for {g.xyz.shape[0]} Gaussians")
+        score, protect = multiview.reduce_blend_weight(score, protect, group)
         rows = train_ops.select_rows(score, budget, protect)
         (g.xyz, g.features_dc, g.features_rest, g.opacity, g.scaling, g.rotation) = self.optimizer.take_rows(rows)
         self.xyz_gradient_accum, self.denom, self.max_radii2D = train_ops.take_rows(

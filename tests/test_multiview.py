@@ -1176,3 +1176,91 @@ def test_bucket_reused_only_when_released_gloo_world2():
         wsum = sum(float(r + 1) * (step + 1) for r in (0, 1))
         for g, x in zip(r0[step][1], prm):
             torch.testing.assert_close(g, 2 * wsum * x, rtol=1e-6, atol=1e-6)
+
+
+def _prune_worker(rank, world, port, out):
+    _init(rank, world, port)
+    import synthetic
+    import train_ops
+    import train_step
+
+    # the kernels' plain forms: what is tested is that the ranks agree
+    def select_rows(score, budget, protect=None):
+        key = score if protect is None else score.masked_fill(protect, float("inf"))
+        return torch.sort(torch.sort(key, descending=True, stable=True).indices[:budget]).values
+
+    def take_rows(tensors, rows, states=None):
+        new = [t.detach()[rows] for t in tensors]
+        return new if states is None else (new, [{k: x if k == "step" else x[rows] for k, x in s.items()} for s in states])
+
+    train_ops.select_rows, train_ops.take_rows = select_rows, take_rows
+    P = 40
+    got = []
+    for protected in (False, True):
+        g = synthetic.make_gaussians(P, 1, seed=0)
+        for p in g.params():
+            p.requires_grad_(True)
+        st = train_step.TrainState(g, 1.0, fused=True, state_bits=32)
+        for p in g.params():
+            st.optimizer.state[p] = {"step": 1, "exp_avg": torch.ones_like(p), "exp_avg_sq": torch.ones_like(p)}
+        score = torch.rand(P, generator=torch.Generator().manual_seed(rank))
+        protect = None
+        if protected and rank == 1:  # one rank's own
+            protect = torch.zeros(P, dtype=torch.bool)
+            protect[:3] = True
+        mine = score.clone()
+        rows = st.prune_to_budget(g, score, 15, protect)
+        assert torch.equal(score, mine)  # the rank's own accumulator is left as it is
+        got.append((rows, [p.detach().clone() for p in g.params()]))
+    out[rank] = got
+    dist.destroy_process_group()
+
+
+def test_prune_to_budget_keeps_the_same_rows_on_every_rank_gloo_world2():
+    """Every rank accumulates the weight of its own views: the rows that stay are those of the sum."""
+    port = _free_port()
+    with mp.Manager() as m:
+        out = m.dict()
+        mp.spawn(_prune_worker, args=(2, port, out), nprocs=2, join=True)
+        res = dict(out)
+    total = sum(torch.rand(40, generator=torch.Generator().manual_seed(r)) for r in (0, 1))
+    for k in (0, 1):
+        key = total.clone()
+        if k == 1:
+            key[:3] = float("inf")
+        want = torch.sort(torch.sort(key, descending=True, stable=True).indices[:15]).values
+        for r in (0, 1):
+            assert torch.equal(res[r][k][0], want), (r, k)
+        assert all(torch.equal(a, b) for a, b in zip(res[0][k][1], res[1][k][1]))
+    assert {0, 1, 2} <= set(res[0][1][0].tolist()) and res[0][0][0].tolist() != res[0][1][0].tolist()
+
+
+def _reduce_weight_worker(rank, world, port, out):
+    _init(rank, world, port)
+    from multiview import reduce_blend_weight
+
+    score = torch.tensor([[1.0], [2.0], [float("nan")]]) * (rank + 1)
+    protect = torch.tensor([rank == 0, False, False]) if rank == 0 else None
+    out[rank] = (reduce_blend_weight(score, protect), reduce_blend_weight(score))
+    for bad in ((score.double(), None), (score, score), (score, torch.zeros(2, dtype=torch.bool))):
+        with pytest.raises(RuntimeError):  # before anything is sent
+            reduce_blend_weight(*bad)
+    dist.destroy_process_group()
+
+
+def test_reduce_blend_weight_gloo_world2():
+    from multiview import reduce_blend_weight
+
+    port = _free_port()
+    with mp.Manager() as m:
+        out = m.dict()
+        mp.spawn(_reduce_weight_worker, args=(2, port, out), nprocs=2, join=True)
+        res = dict(out)
+    for r in (0, 1):
+        (s, p), (s2, p2) = res[r]
+        assert s.shape == (3, 1) and s[:2, 0].tolist() == [3.0, 6.0] and torch.isnan(s[2, 0])
+        assert p.tolist() == [True, False, False] and not p2.any() and torch.equal(s[:2], s2[:2])
+    # without a process group: the rank's own
+    score, protect = torch.rand(4), torch.zeros(4, dtype=torch.bool)
+    s, p = reduce_blend_weight(score, protect)
+    assert torch.equal(s, score) and p is protect and reduce_blend_weight(score)[1] is None
