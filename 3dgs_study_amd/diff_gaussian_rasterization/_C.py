@@ -270,6 +270,16 @@ def load_library():
             f"diff_gaussian_rasterization: native library {path} not found; build it with "
             "`python -c 'import __graft_entry__; __graft_entry__.build()'` (hipcc --offload-arch=gfx950)")
     lib = ctypes.CDLL(str(path))
+    # before any signature is set: a library of another build is refused by its version, or by what it lacks
+    # (entry points are added without a new version, which stands for the structures' layouts)
+    if not hasattr(lib, "gsr_abi_version"):
+        raise ImportError(f"{path}: no gsr_abi_version; rebuild")
+    lib.gsr_abi_version.restype = ctypes.c_int
+    if lib.gsr_abi_version() != ABI_VERSION:
+        raise ImportError(f"{path}: ABI version {lib.gsr_abi_version()} != {ABI_VERSION}; rebuild")
+    missing = [name for name in EXPORTED if not hasattr(lib, name)]
+    if missing:
+        raise ImportError(f"{path}: no {', '.join(missing)}; rebuild")
     sz, i32, i64, vp = ctypes.c_size_t, ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
     lib.gsr_geom_bytes.argtypes = [i32, i32, i32]
     lib.gsr_geom_bytes.restype = sz
@@ -365,10 +375,7 @@ def load_library():
     lib.gsr_knn_mean_dist2.argtypes = [i32, vp, vp, vp, vp]
     lib.gsr_knn_mean_dist2.restype = ctypes.c_int
     lib.gsr_last_error.restype = ctypes.c_char_p
-    lib.gsr_abi_version.restype = ctypes.c_int
     lib.gsr_build_id.restype = ctypes.c_char_p
-    if lib.gsr_abi_version() != ABI_VERSION:
-        raise ImportError(f"{path}: ABI version {lib.gsr_abi_version()} != {ABI_VERSION}; rebuild")
     if os.environ.get("GSR_COLOUR_APART"):  # preprocess's colour half on a side stream (set_colour_apart)
         if lib.gsr_colour_mode(int(os.environ["GSR_COLOUR_APART"])) < -1:
             raise ImportError(f"GSR_COLOUR_APART={os.environ['GSR_COLOUR_APART']!r}: {lib.gsr_last_error().decode()}")

@@ -380,3 +380,25 @@ def test_colour_mode_values():
         assert _C.get_colour_mode() == 1
     finally:
         _C.set_colour_mode(prev)
+
+
+def test_a_library_that_lacks_an_entry_point_says_rebuild(tmp_path, monkeypatch):
+    """An older build with the same structure layouts: refused by name, as one of another layout is."""
+    import subprocess
+
+    from diff_gaussian_rasterization import _C
+
+    def build(name, entries, version):
+        src = tmp_path / f"{name}.c"
+        src.write_text("".join(f"int {n}(void) {{ return {version}; }}\n" for n in entries))
+        subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(tmp_path / f"{name}.so"), str(src)], check=True)
+        monkeypatch.setenv("GSR_LIBRARY", str(tmp_path / f"{name}.so"))
+
+    monkeypatch.setattr(_C, "_lib", None)
+    build("older", [n for n in _C.EXPORTED if n != "gsr_take_rows"], _C.ABI_VERSION)
+    with pytest.raises(ImportError, match="gsr_take_rows.*rebuild"):
+        _C.load_library()
+    build("other", ["gsr_abi_version"], _C.ABI_VERSION - 1)
+    with pytest.raises(ImportError, match="ABI version.*rebuild"):
+        _C.load_library()
+    assert _C._lib is None
