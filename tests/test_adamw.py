@@ -978,3 +978,70 @@ def test_train_state_decays_the_groups_that_are_named():
         train_step.TrainState(g, 1.0, fused=True, weight_decay={"positions": 0.1})
     with pytest.raises(ValueError, match="fused"):
         train_step.TrainState(g, 1.0, weight_decay={"f_rest": 0.1})
+
+
+# ------------------------------------------------------------------ GPU: bit for bit
+RCP = {32: False, 8: True}  # whose quotient is a product with the hardware's reciprocal
+
+
+def _fp32_step(p, g, m, v, lr, wd, t, c=1.0, rcp=False, betas=(0.9, 0.999), eps=1e-15):
+    """(all the values that p' may have, m', v') by the formulas in numpy's fp32, where each operation
+    rounds once (torch's square root on the CPU does not round to nearest).  ``rcp``: the quotient
+    is a product with a reciprocal that is off by one ulp at most, so its value to nearest or one
+    of the two numbers next to it; else it rounds once itself."""
+    f, (b1, b2) = np.float32, betas
+    p, g, m, v = (x.float().numpy() for x in (p, g, m, v))
+    x = g * f(c)
+    m2, v2 = m + (x - m) * f(1 - b1), v * f(b2) + (x * x) * f(1 - b2)
+    d = np.sqrt(v2) * f(1 / math.sqrt(1 - b2 ** t)) + f(eps)
+    if rcp:
+        r = f(1) / d
+        quotients = [m2 * y for y in (r, np.nextafter(r, f(0)), np.nextafter(r, f(np.inf)))]
+    else:
+        quotients = [m2 / d]
+    ps = [p * f(1 - lr * wd) + q * f(-lr / (1 - b1 ** t)) for q in quotients]
+    assert all(y.dtype == f for y in ps + [m2, v2])
+    return [torch.from_numpy(y) for y in ps], torch.from_numpy(m2), torch.from_numpy(v2)
+
+
+def _dithered(p2, words):
+    """Rounded to bf16 by 16 bits formed of the element's word: up where the dropped bits and they carry."""
+    low = (((words * 0x9E3779B9) & M32) >> 16).to(torch.int32)
+    return ((p2.view(torch.int32) + low) & -0x10000).view(torch.float32).bfloat16()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("clip", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_step_bit_for_bit(dev, dtype, clip, bits):
+    """Parameters and 32-bit moments are those of the formulas in fp32, each operation rounded by
+    itself; a bf16 parameter is rounded by the documented random bits."""
+    import train_ops
+
+    seed, sizes = 0xFEDC_BA98_7654_3210, SIZES + [100_003]
+    ins = [_inputs(n, n + 2, dtype) for n in sizes]
+    P, G = [i[0].to(dev) for i in ins], [i[1].to(dev) for i in ins]
+    st = [_state8(i[2], i[3], dev) if bits == 8 else {"exp_avg": i[2].to(dev), "exp_avg_sq": i[3].to(dev)} for i in ins]
+    old = [{k: x.cpu() for k, x in s.items() if k != "step"} for s in st]
+    for k, s in enumerate(st):
+        s["step"] = 7 * k
+    c, scale = 1.0, None
+    if clip:
+        _, scale = train_ops.grad_norm(G, 1e-6)
+        c = float(scale)
+    train_ops.adamw_step(P, G, st, 0.01, 0.1, grad_scale=scale, seed=seed)
+    for k, (p, g, m, v) in enumerate(ins):
+        n, t = sizes[k], 7 * k + 1
+        words = _words(n, seed, t, k)
+        if bits == 8:
+            m = _values(old[k]["exp_avg"], old[k]["exp_avg_scale"]).float()
+            r = _values(old[k]["exp_rms"], old[k]["exp_rms_scale"]).float()
+            v = r * r
+        want, m2, v2 = _fp32_step(p, g, m, v, 0.01, 0.1, t, c, rcp=RCP[bits])
+        if bits == 32:
+            assert torch.equal(st[k]["exp_avg"].cpu(), m2) and torch.equal(st[k]["exp_avg_sq"].cpu(), v2), n
+        if dtype is torch.bfloat16:
+            want = [_dithered(w, words) for w in want]
+        hit = torch.stack([P[k].cpu() == w for w in want]).any(0)
+        assert bool(hit.all()), (n, int((~hit).sum()))
