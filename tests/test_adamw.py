@@ -1045,3 +1045,45 @@ def test_step_bit_for_bit(dev, dtype, clip, bits):
             want = [_dithered(w, words) for w in want]
         hit = torch.stack([P[k].cpu() == w for w in want]).any(0)
         assert bool(hit.all()), (n, int((~hit).sum()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_bf16_rounding_is_unbiased(dev, bits):
+    """(rounded - exact) / step over N elements lies in (-1, 1) with mean 0 and variance at most
+    1/4: six standard deviations are 3 / sqrt(N); every one of the 2^16 dropped patterns has
+    its own share of the 2^16 random ones, so there is no bias but the fp32 value's own error, far
+    below 2^-10 of a step."""
+    import train_ops
+
+    n = 1 << 18
+    p, g, m, v = _inputs(n, 11, torch.bfloat16)
+    st = {"step": 50, "exp_avg": m.to(dev), "exp_avg_sq": v.to(dev)} if bits == 32 else {**_state8(m, v, dev), "step": 50}
+    if bits == 8:
+        m = _values(st["exp_avg"].cpu(), st["exp_avg_scale"].cpu())
+        v = _values(st["exp_rms"].cpu(), st["exp_rms_scale"].cpu()) ** 2
+    P = p.to(dev)
+    train_ops.adamw_step([P], [g.to(dev)], [st], 0.01, 0.1, seed=3)
+    want = _exact(p, g, m, v, 0.01, 0.1, 51)[0][0]
+    step = torch.exp2(torch.frexp(want)[1].double() - 8)
+    err = (P.cpu().double() - want) / step
+    assert float(err.abs().max()) < 1 + 2.0 ** -10
+    assert float((err != 0).float().mean()) > 0.9
+    assert abs(float(err.mean())) <= 3 / math.sqrt(n) + 2.0 ** -10
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_bf16_parameters_follow_updates_far_below_half_a_step(dev, bits):
+    """From zero moments the first update is lr g / |g|.  Of 1.5 (steps of 2^-7) an lr of 2^-13
+    moves one element in 64 by a whole step: the mean of N moves by 2^-13, with a standard deviation
+    of 2^-7 sqrt(63) / 64 / sqrt(N) < 2^-19; rounded to nearest none would move."""
+    import train_ops
+
+    n = 1 << 18
+    p = torch.full((n,), 1.5, dtype=torch.bfloat16, device=dev)
+    g = torch.full((n,), 1e-3, dtype=torch.bfloat16, device=dev)
+    train_ops.adamw_step([p], [g], [train_ops.adamw_state(p, bits)], 2.0 ** -13, seed=9)
+    assert set(p.unique().tolist()) == {1.5, 1.5 - 2.0 ** -7}
+    # the update itself: 14 u of 2^-13
+    assert abs(1.5 - float(p.double().mean()) - 2.0 ** -13) <= 6 * 2.0 ** -19 + 14 * U * 2.0 ** -13
