@@ -157,6 +157,12 @@ def _on(device):
     return _SAME if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+def _raw_stream(index: int) -> int:
+    """The current stream's handle on device ``index``: as _C._stream, without the 2 us of a
+    torch.cuda.Stream object, a tenth of a small step."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def adamw_state(param: torch.Tensor, state_bits: int = 32) -> dict:
     """The initial AdamW state of a tensor.  32 bits: ``exp_avg`` and ``exp_avg_sq`` in
     float32, as torch's.  8 bits: ``exp_avg`` and ``exp_rms`` (the root of exp_avg_sq) as
@@ -309,7 +315,7 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
             raise RuntimeError("adamw_step: step counts and rates are host values; not for graph capture")
         if grad_scale is not None:
             grad_scale = grad_scale.resolve_neg()
-        stream, scale = _C._stream(dev), None if grad_scale is None else grad_scale.data_ptr()
+        stream, scale = _raw_stream(at), None if grad_scale is None else grad_scale.data_ptr()
         seed &= 0xFFFFFFFFFFFFFFFF
         tables = [(kind, struct.pack("7q2d2i" * (len(segs) // 11), *segs), len(segs) // 11)  # gsr_adamw_segment
                   for kind, segs in launches.items()]
@@ -344,7 +350,7 @@ def grad_norm(grads, max_norm: float = math.inf):
         out = torch.empty(2, dtype=torch.float32, device=dev)
         scratch = torch.empty(lib.gsr_grad_norm_scratch_bytes(count), dtype=torch.uint8, device=dev)
         _C._check(lib.gsr_grad_norm(struct.pack("3q" * count, *segs), count, float(max_norm), scratch.data_ptr(),
-                                    out.data_ptr(), _C._stream(dev)), "gsr_grad_norm")
+                                    out.data_ptr(), _raw_stream(at)), "gsr_grad_norm")
     return out.unbind()
 
 
@@ -502,7 +508,7 @@ def select_rows(score: torch.Tensor, budget: int, protect: torch.Tensor = None) 
         if rows.numel():
             scratch = torch.empty(lib.gsr_select_rows_scratch_bytes(P), dtype=torch.uint8, device=dev)
             _C._check(lib.gsr_select_rows(s.data_ptr(), None if pr is None else pr.data_ptr(), P, rows.numel(),
-                                          rows.data_ptr(), scratch.data_ptr(), _C._stream(dev)), "gsr_select_rows")
+                                          rows.data_ptr(), scratch.data_ptr(), _raw_stream(dev.index)), "gsr_select_rows")
     return rows
 
 
@@ -576,7 +582,7 @@ def take_rows(tensors, rows: torch.Tensor, states=None):
         if K and segs:
             count = len(segs) // 6  # gsr_rows_segment's fields, the last two as one
             _C._check(lib.gsr_take_rows(struct.pack(f"{6 * count}q", *segs), count, P, rows.data_ptr(), K,
-                                        _C._stream(dev)), "gsr_take_rows")
+                                        _raw_stream(at)), "gsr_take_rows")
     return out if states is None else (out, new_states)
 
 
