@@ -354,8 +354,9 @@ def grad_norm(grads, max_norm: float = math.inf):
     return out.unbind()
 
 
-def _adamw_options(groups) -> tuple:
-    """(betas, eps) of the param groups, which share them; what a step would not do is refused."""
+def _adamw_options(groups, betas, eps) -> tuple:
+    """(betas, eps) of the param groups, which share them (those given where a group has none); what a
+    step would not do is refused."""
     got = set()
     for g in groups:
         for k in ("amsgrad", "maximize"):
@@ -363,11 +364,11 @@ def _adamw_options(groups) -> tuple:
                 raise ValueError(f"FusedAdamW: {k} is not implemented")
         if g["weight_decay"] and not g.get("decoupled_weight_decay", True):
             raise ValueError("FusedAdamW: weight decay is decoupled (a checkpoint of torch.optim.Adam's is not)")
-        b1, b2 = g["betas"]
-        got.add(((float(b1), float(b2)), float(g["eps"])))
+        b1, b2 = g.get("betas", betas)
+        got.add(((float(b1), float(b2)), float(g.get("eps", eps))))
     if len(got) > 1:
         raise ValueError(f"FusedAdamW: all groups have the same betas and eps (got {sorted(got)})")
-    return got.pop() if got else None
+    return got.pop() if got else (betas, eps)
 
 
 class FusedAdamW:
@@ -388,24 +389,28 @@ class FusedAdamW:
             g.setdefault("weight_decay", weight_decay)
             g.setdefault("betas", tuple(betas))
             g.setdefault("eps", eps)
-        _adamw_options(self.param_groups)
+        self._defaults = {"betas": tuple(betas), "eps": eps}
+        self._options()
         self.state_bits, self.max_norm, self.seed = state_bits, max_norm, seed
         self.state = {}
         self.grad_norm = None
 
+    def _options(self) -> tuple:
+        return _adamw_options(self.param_groups, **self._defaults)
+
     def _set_option(self, key, value):
-        for g in self.param_groups:
+        for g in [self._defaults] + self.param_groups:
             g[key] = value
 
-    betas = property(lambda self: _adamw_options(self.param_groups)[0], lambda self, b: self._set_option("betas", tuple(b)))
-    eps = property(lambda self: _adamw_options(self.param_groups)[1], lambda self, e: self._set_option("eps", e))
+    betas = property(lambda self: self._options()[0], lambda self, b: self._set_option("betas", tuple(b)))
+    eps = property(lambda self: self._options()[1], lambda self, e: self._set_option("eps", e))
 
     @torch.no_grad()
     def step(self):
         todo = [(g, p) for g in self.param_groups for p in g["params"] if p.grad is not None]
         if not todo:
             return
-        betas, eps = _adamw_options(self.param_groups)
+        betas, eps = self._options()
         params = [p for _, p in todo]
         grads = [p.grad for p in params]
         states = [self.state[p] if p in self.state else adamw_state(p, self.state_bits) for p in params]
@@ -439,7 +444,7 @@ class FusedAdamW:
         if [len(g["params"]) for g in d["param_groups"]] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("FusedAdamW.load_state_dict: other param groups")
         groups = [{**g, **{n: x for n, x in h.items() if n != "params"}} for g, h in zip(self.param_groups, d["param_groups"])]
-        _adamw_options(groups)
+        betas, eps = _adamw_options(groups, **self._defaults)
         state_bits = d.get("state_bits", self.state_bits)
         if state_bits not in _KEYS:
             raise ValueError(f"FusedAdamW.load_state_dict: state_bits must be 32 or 8 (got {state_bits})")
@@ -452,6 +457,7 @@ class FusedAdamW:
             _state_ptrs(st, p, p.numel(), "FusedAdamW.load_state_dict")
             state[p] = st
         self.state, self.state_bits = state, state_bits
+        self._defaults = {"betas": betas, "eps": eps}
         self.seed, self.max_norm = d.get("seed", self.seed), d.get("max_norm", self.max_norm)
         for g, h in zip(self.param_groups, groups):
             g.update(h)

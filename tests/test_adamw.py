@@ -901,6 +901,16 @@ def test_state_dict_holds_all_that_a_step_depends_on():
     assert all(g["betas"] == (0.7, 0.95) and g["eps"] == 1e-9 for g in b.param_groups)
 
 
+def test_a_group_without_betas_goes_by_the_optimisers():
+    import train_ops
+
+    _, opt = _adamw_on_cpu(betas=(0.8, 0.9))
+    opt.param_groups.append({"params": [torch.ones(1)], "lr": 0.1, "weight_decay": 0.0})
+    assert opt.betas == (0.8, 0.9) and opt.eps == 1e-15
+    opt.betas = (0.5, 0.6)
+    assert opt.betas == (0.5, 0.6) and train_ops.FusedAdamW([], eps=1e-3).eps == 1e-3
+
+
 @pytest.mark.parametrize("change, msg", [(dict(amsgrad=True), "amsgrad"), (dict(maximize=True), "maximize"),
                                          (dict(betas=(0.5, 0.9)), "betas"), (dict(eps=1e-3), "eps"),
                                          (dict(decoupled_weight_decay=False, weight_decay=0.1), "decoupled")])
