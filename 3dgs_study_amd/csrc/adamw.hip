@@ -14,9 +14,9 @@
 // kernel's arguments (40 tensors a launch), so nothing is uploaded and nothing is kept.
 // Memory bounds it: 28 bytes an element with 32-bit states, 16 with 8-bit ones.  59M
 // elements (1M Gaussians): 265 us = 6.2 TB/s and 150 us = 6.3 TB/s, where a large copy
-// reaches 4.75 and an addition of two arrays 5.85.  All of it streams non-temporally: 304
-// us (32 bits) with ordinary accesses, 274 with the parameters alone kept in the caches (too
-// large to be there at the next render).  Two or four vectors a lane: 314, 316 us.
+// reaches 4.8 and an addition of two arrays 5.85.  All of it streams non-temporally: 306
+// us (32 bits) with ordinary accesses, 277 with the parameters alone kept in the caches (too
+// large to be there at the next render).  Two or four vectors a lane: 282, 282 us.
 //
 // 8-bit states hold m and r = sqrt(v) (half the range of v's exponents) as e4m3 codes
 // with a power-of-two scale for every 64 elements (gsr_blockscale.hpp).  They are
@@ -24,8 +24,9 @@
 // (1 - b2) = 0.1 %, so rounding to nearest would never let a second moment fall, and
 // would hold the first moments of Gaussians that no view sees at their last few codes,
 // which then drift for ever.  The parameter is updated from the fp32 moments before
-// they are rounded.  Arithmetic was the bound at 95 instructions an element (165 us);
-// with the test for infinities and NaN made once a wave, 75 leave it to memory (150 us).
+// they are rounded.  75 instructions an element leave it to memory, with the test for
+// infinities and NaN made once a wave (for every element: 157 us instead of 153).  With bf16
+// parameters, 87 instructions for 10 bytes, arithmetic bounds it: 125 us = 4.8 TB/s.
 //
 // Parameters and gradients are fp32 or bf16; a bf16 parameter is rounded
 // stochastically too (an update below 2^-9 of the parameter would be lost).
@@ -299,11 +300,14 @@ hipError_t launch_adamw(const gsr_adamw_segment *segs, int nseg, int dtype, int 
 // ------------------------------------------------------------ global gradient norm
 //
 // norm = sqrt(sum g^2) over all tensors, c = min(1, max_norm / (norm + 1e-6)).  Squares
-// and sums in 64 bits (the fp64 rate is far above what the stream of gradients needs):
-// no overflow, and the same value whatever the split.  Each workgroup leaves one partial
-// sum; one workgroup adds them in a fixed order.  1180 MB in 192 us = 6.1 TB/s (2048
-// workgroups: 208).  The loads stay in the caches, for the step that follows: read
-// non-temporally, both together cost 406 us instead of 385 (177 MB of bf16 gradients).
+// and sums in 64 bits (the fp64 rate is far above what the stream of gradients needs): no
+// overflow, the same bits for the same list of tensors, and for another split of the same
+// values a sum that may differ in the last of its 53 bits.  Each workgroup leaves one partial
+// sum; one workgroup adds them in a fixed order.  1180 MB in 193 us = 6.1 TB/s; 177 MB of 96
+// bf16 tensors in 47 us = 3.8 TB/s: ten 16 KB tiles a workgroup, each behind a search of the table
+// and its own loads.  2048 workgroups: 266 us instead of 249 a call for the large one, behind 1
+// GB of writes.  The loads stay in the caches, for the step that follows: read non-temporally,
+// both together cost 404 us instead of 385 (the 177 MB).
 constexpr int GN_THREADS = 256, GN_SEGS = 128, GN_BLOCKS = 1024, GN_UNROLL = 4;
 constexpr int64_t gn_tile(int dtype) { return GN_THREADS * GN_UNROLL * (dtype == GSR_DTYPE_F32 ? 4 : 8); }  // 16 KB
 struct NormArgs {

@@ -67,8 +67,8 @@ __device__ __forceinline__ uint32_t e4m3_stochastic(float x, uint32_t byte, uint
     return SIGNED ? c | ((bits >> 24) & 0x80u) : c;
 }
 
-// A 32-bit mixing (xor-shifts and odd multipliers: the fractional bits of the roots of
-// 2 and 3), and the random word of element i of a tensor from the tensor's key: a pure
+// A 32-bit mixing of the published xor-shift-multiply form (shifts by 16, 15 and 16 around
+// two odd multipliers; these are the fractional bits of the roots of 2 and 3), and the random word of element i of a tensor from the tensor's key: a pure
 // function, so a run repeats and every replica of a data-parallel job rounds alike.
 __host__ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
     x ^= x >> 16;

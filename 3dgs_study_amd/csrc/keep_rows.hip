@@ -9,7 +9,8 @@
 // The kept rows are then counted per tile, the counts scanned, and the indices written in
 // order.  All counts are integers: the result does not depend on the order of the atomics.
 // Six launches, 37 us for 1M scores and 53 us for 5M (the scores are read five times, from
-// the caches); up to 16384 scores one workgroup does it all (10k: 14 us, 28 us by the six).
+// the caches): each waits for the one before it, 2-8 us at any size up to 1M.  Up to 16384
+// scores one workgroup does it all (10k: 14 us, the six 23 us and the gaps between them).
 #include "gsr_blockscale.hpp"
 #include "gsr_kernels.hpp"
 #include "gsr_wave.hpp"
@@ -98,9 +99,10 @@ __device__ __forceinline__ void pass_state(const SelectArgs &a, uint32_t *sh, ui
 }
 
 // Few workgroups of 16 waves: each ends in one atomic per bin that it met, and with 1024
-// workgroups of four waves those were most of the pass (5M scores: 20 us a pass, now 10).
-// Scores gather in few bins (their exponents), so every bin has SR_COPIES counters, one
-// for every eighth lane, which keeps a wave's additions apart.
+// workgroups of four waves those are most of the pass (5M scores: 24 us the first pass
+// instead of 10).  Where scores share a bin (equal ones), a wave's additions to one counter
+// follow each other: every bin has SR_COPIES counters, one for every eighth lane (5M equal
+// scores: 8 us a pass, 22 with one counter; scores that spread: the same).
 template <int D>
 __global__ void __launch_bounds__(SR_HIST_THREADS) select_hist_kernel(SelectArgs a) {
     __shared__ uint32_t h[SR_BINS * SR_COPIES], sh[32];
@@ -165,8 +167,7 @@ __global__ void __launch_bounds__(SR_THREADS) select_write_kernel(SelectArgs a) 
         eq0 = block_sum<SR_THREADS>(eq0, sh);
     }
     // keys above T in the low half, equal to T in the high half (4096 each at most); the kept
-    // places are lined up in LDS and leave in one run (stored one by one from the lanes that
-    // keep them: 15 us for 5M scores, now 13)
+    // places are lined up in LDS and leave in one run (13 us for 5M scores)
     __shared__ uint16_t kept[SR_TILE];
     const int64_t tile0 = (int64_t)blockIdx.x * SR_TILE;
     uint32_t gt = 0, eq = eq0;
@@ -290,17 +291,17 @@ hipError_t launch_select_rows(const float *score, const uint8_t *protect, int P,
 // leave the source (its first and last rows) the lane reads its bytes one by one.  Rows that
 // are too short for it (4-byte rows: opacities) move one unit a lane.
 // Memory bounds it, counted in whole lines, those of dropped rows among them: 1M -> 500k
-// Gaussians with fp32 states 152 us (unit by unit: 198), 5M -> 3M with 8-bit states 600 us
-// (3.1 GB moved, 5.1 TB/s; a byte or a word of codes a lane: 850 us).  Stored non-temporally
-// (164 -> 152 us), loaded through the caches, which hold the neighbouring rows' part of a line.
+// Gaussians with fp32 states 152 us, 5M -> 3M with 8-bit states 600 us (3.1 GB moved, 5.1
+// TB/s).  Stored non-temporally (161 -> 152 us), loaded through the caches, which hold the
+// neighbouring rows' part of a line.
 //
 // 8-bit states (gsr_blockscale.hpp): the rows' values land in other blocks of 64, whose
 // scale is formed anew from what they hold; powers of two, so only values below 2^-13 of
 // their new block's largest lose bits.
 constexpr int TR_THREADS = 256, TR_SEGS = 40, TR_ITEMS = 8, TR_SPANS = 2;
 constexpr int TR_TILE = TR_THREADS * TR_ITEMS;        // units per workgroup, unit by unit
-constexpr int TR_BYTES = TR_THREADS * TR_SPANS * 16;  // bytes or codes per workgroup in spans (four a lane: codes 385
-                                                      // instead of 328 us, in 92 registers instead of 53)
+constexpr int TR_BYTES = TR_THREADS * TR_SPANS * 16;  // bytes or codes per workgroup in spans (four spans a lane: 677
+                                                      // instead of 606 us at 5M -> 3M with 8-bit states)
 
 struct TakeSeg {
     const void *src;

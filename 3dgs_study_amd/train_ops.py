@@ -266,13 +266,13 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
     ``lr`` and ``weight_decay``: a number, or one per tensor.  Each state's ``step`` counts
     its own tensor's steps and is advanced by one.  ``grad_scale``: a float32 scalar on the
     device that every gradient is multiplied by (``grad_norm``'s second result).  Parameters
-    are float32 or bfloat16, gradients of the same dtype, all contiguous and on one device, parameters
-    and states no negated views.
+    are float32 or bfloat16, gradients of the same dtype, all contiguous and on one device;
+    parameters and states are no negated views.
     8-bit states and bfloat16 parameters are rounded stochastically, by a pure function of
     ``seed`` (an int of up to 64 bits), the tensor's step, its place in the list and the
-    element: the same call gives the same bits.  Tensors must not overlap.  Step counts,
-    rates and seed are host values and would be frozen in a captured graph: under capture
-    this raises.
+    element: the same call gives the same bits.  ``eps``: 0, or 2^-126 and above.  Tensors must
+    not overlap.  Step counts, rates and seed are host values and would be frozen in a captured
+    graph: under capture this raises.
 
     Everything is validated before anything is launched and any count advanced."""
     lib = _C.load_library()
@@ -331,7 +331,8 @@ def grad_norm(grads, max_norm: float = math.inf):
     """(norm, scale), two float32 scalars on the device: the 2-norm over all the tensors
     (float32 or bfloat16; squares and sums in 64 bits), and ``min(1, max_norm / (norm +
     1e-6))``, torch.nn.utils.clip_grad_norm_'s coefficient, which ``adamw_step`` takes as
-    ``grad_scale``.  The gradients are not written and the host does not wait."""
+    ``grad_scale`` (as torch's, NaN where the norm and ``max_norm`` are both infinite).  The gradients
+    are not written and the host does not wait."""
     lib = _C.load_library()
     if not len(grads):
         raise ValueError("grad_norm: no gradients")
@@ -519,12 +520,13 @@ def select_rows(score: torch.Tensor, budget: int, protect: torch.Tensor = None) 
 
 
 def take_rows(tensors, rows: torch.Tensor, states=None):
-    """``[t[rows] for t in tensors]`` in one launch for up to 48 tensors of any dtype, as new
-    tensors without gradient history.  ``rows``: int64 [K], any order, repeats allowed; an index
-    outside [0, P) gives a row of zeros (-1: a fresh row).  With ``states`` (AdamW state dicts of
-    tensors with P rows, ``adamw_state``) returns (tensors, states): the states' rows, with
-    ``step`` kept; 8-bit values are re-blocked under new scales, which changes a value only
-    where it is below 2^-13 of its new block's largest."""
+    """``[t[rows] for t in tensors]`` for tensors of any dtype, as new tensors of up to 2^34 bytes
+    each (2^33 of an 8-bit state) without gradient history.  ``rows``: int64 [K], any order,
+    repeats allowed; an index outside [0, P) gives a row of zeros (-1: a fresh row).  With
+    ``states`` (AdamW state dicts of tensors with P rows, ``adamw_state``) returns (tensors,
+    states): the states' rows, with ``step`` kept; 8-bit values are re-blocked under new scales,
+    which changes a value only where it is below 2^-13 of its new block's largest.  One launch
+    takes up to 40 tensors, where a state counts as two."""
     lib = _C.load_library()
     if rows.dtype is not torch.int64 or rows.dim() != 1 or not rows.is_cuda:
         raise RuntimeError(f"take_rows: rows must be an int64 vector on the GPU, got {rows.dtype} {tuple(rows.shape)} "

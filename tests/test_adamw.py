@@ -1097,3 +1097,18 @@ def test_bf16_parameters_follow_updates_far_below_half_a_step(dev, bits):
     assert set(p.unique().tolist()) == {1.5, 1.5 - 2.0 ** -7}
     # the update itself: 14 u of 2^-13
     assert abs(1.5 - float(p.double().mean()) - 2.0 ** -13) <= 6 * 2.0 ** -19 + 14 * U * 2.0 ** -13
+
+
+@pytest.mark.gpu
+def test_grad_norm_infinite_norm_and_bound(dev):
+    """As torch's clipping: an infinite norm over an infinite bound is NaN; a finite one is not scaled."""
+    import train_ops
+
+    g = torch.tensor([1.0, math.inf], device=dev)
+    norm, scale = train_ops.grad_norm([g], math.inf)
+    assert math.isinf(float(norm)) and math.isnan(float(scale))
+    assert float(train_ops.grad_norm([g[:1]], math.inf)[1]) == 1.0
+    p = torch.ones(2, device=dev, requires_grad=True)
+    p.grad = g.clone()
+    torch.nn.utils.clip_grad_norm_([p], math.inf)
+    assert bool(torch.isnan(p.grad).all())
