@@ -290,7 +290,7 @@ def adamw_step(params, grads, states, lr, weight_decay=0.0, betas=(0.9, 0.999), 
                 not p.is_same_size(g) or not (p.is_contiguous() and g.is_contiguous()) or \
                 dt is _F32 and p.is_neg():
             _adamw_refuse(p, g, dev)
-        if dt is _F32 and g.is_neg():  # as a conjugated complex number's imaginary part leaves it: its bytes are not its values
+        if dt is _F32 and g.is_neg():  # as a conjugated complex number's backward leaves it
             g = g.resolve_neg()
             keep.append(g)  # until the launch
         size = p.numel()
@@ -444,7 +444,8 @@ class FusedAdamW:
         Options that a step would not follow (amsgrad, maximize, betas by group) are refused."""
         if [len(g["params"]) for g in d["param_groups"]] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("FusedAdamW.load_state_dict: other param groups")
-        groups = [{**g, **{n: x for n, x in h.items() if n != "params"}} for g, h in zip(self.param_groups, d["param_groups"])]
+        groups = [{**g, **{n: x for n, x in h.items() if n != "params"}}
+                  for g, h in zip(self.param_groups, d["param_groups"])]
         betas, eps = _adamw_options(groups, **self._defaults)
         state_bits = d.get("state_bits", self.state_bits)
         if state_bits not in _KEYS:
@@ -515,7 +516,8 @@ def select_rows(score: torch.Tensor, budget: int, protect: torch.Tensor = None) 
         if rows.numel():
             scratch = torch.empty(lib.gsr_select_rows_scratch_bytes(P), dtype=torch.uint8, device=dev)
             _C._check(lib.gsr_select_rows(s.data_ptr(), None if pr is None else pr.data_ptr(), P, rows.numel(),
-                                          rows.data_ptr(), scratch.data_ptr(), _raw_stream(dev.index)), "gsr_select_rows")
+                                          rows.data_ptr(), scratch.data_ptr(), _raw_stream(dev.index)),
+                      "gsr_select_rows")
     return rows
 
 

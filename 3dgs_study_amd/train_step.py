@@ -335,7 +335,8 @@ class TrainState:
         if adamw and not fused:
             raise ValueError("TrainState: state_bits, weight_decay and max_norm need fused=True")
         if seed and not adamw:
-            raise ValueError("TrainState: seed needs state_bits, weight_decay or max_norm (nothing else is rounded at random)")
+            raise ValueError("TrainState: seed needs state_bits, weight_decay or max_norm (nothing else is "
+                             "rounded at random)")
         if isinstance(weight_decay, dict):
             unknown = set(weight_decay) - {group["name"] for group in groups}
             if unknown:
